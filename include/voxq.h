@@ -117,6 +117,9 @@ VOXQ_API VoxCPMError tensor_cuda_upload_weight(Tensor** t_ptr);
 
 /* Block formats: the codes of scripts/quantize.py:28 (QUANT_TYPES). */
 enum { VOXQ_F32 = 0, VOXQ_F16 = 1, VOXQ_Q4 = 2, VOXQ_Q8 = 3 };
+/* bfloat16, an element type of the batched-step operators only (4 is free in
+ * quantize.py's table; the VXCP container's dtype codes are a separate set). */
+enum { VOXQ_BF16 = 4 };
 #define VOXQ_BLOCK 32
 
 /* Library version string. */
@@ -476,6 +479,162 @@ typedef struct {
     int patch_size;
 } voxq_locenc_desc;
 VOXQ_API VoxCPMError voxq_locenc_forward(const voxq_locenc_desc* enc, const Tensor* audio_feats, Tensor* out);
+
+/* ---- A decoder step over many utterances ---------------------------------
+ * Operators for a ragged batch of sequences, each with its own number of new
+ * tokens (one per step, a chunk, a whole prompt).  The reference runs one
+ * sequence at a time (src/model.c:653) and has none of them.  The tokens of
+ * all sequences are concatenated: sequence s owns rows cu[s] .. cu[s+1] - 1,
+ * cu[0] = 0 (device int32 [batch + 1]; a sequence may own none).
+ *
+ * All pointers are device pointers, all calls are asynchronous on `stream`,
+ * allocate nothing and can be captured into a CUDA graph.  Element types are
+ * VOXQ_F32, VOXQ_F16 and VOXQ_BF16; sums, softmax statistics and norms are
+ * fp32.  Strides are in elements; the last dimension is contiguous; base
+ * addresses and strides must be multiples of 16 bytes where a comment says
+ * "16-byte rows".  Results are the same bits on every run (no atomics).
+ * VOXCPM_ERR_INTERNAL: a NULL pointer or a failed launch; _SHAPE_MISMATCH:
+ * negative or contradictory sizes; _UNSUPPORTED: an element type, size or
+ * alignment that the kernels do not take; _OOM: a workspace below the size
+ * that the workspace function gives.  Integer inputs on the device (cu,
+ * lengths, tables, positions, slots, indices) cannot be checked by the host:
+ * the kernels clamp every address that they make from them, so wrong values
+ * give wrong results but no access outside the buffers described here. */
+
+/* Rotary tables: out[p][i] = (cos, sin) of p * f_i * attn_factor-scaled, for
+ * p < n_pos and i < rot_dim / 2 -- the layout of the engine's freqs_cis
+ * (src/tensor.c:883-950) -- with angles in fp64 and
+ *   f_i = theta^(-2 i / rot_dim)                              VOXQ_ROPE_PLAIN
+ *   f_i / factor                                              VOXQ_ROPE_LINEAR
+ *   (theta factor^(rot_dim / (rot_dim - 2)))^(-2 i / rot_dim) VOXQ_ROPE_NTK
+ *   f_i (1 - g_i) / factor + f_i g_i                          VOXQ_ROPE_YARN
+ *   f_i / long_factors[i]                                     VOXQ_ROPE_LONG
+ * where g_i = 1 - clamp((i - lo) / (hi - lo), 0, 1), lo and hi the (floored /
+ * ceiled, clamped to [0, rot_dim - 1]) indices at which a pair turns beta_fast and beta_slow times
+ * within original_len positions: i(b) = rot_dim ln(original_len / (2 pi b)) /
+ * (2 ln theta).  Both cos and sin are multiplied by attn_factor (1 if 0 is
+ * given; YaRN's 0.1 ln(factor) + 1 is the caller's choice). */
+enum { VOXQ_ROPE_PLAIN = 0, VOXQ_ROPE_LINEAR = 1, VOXQ_ROPE_NTK = 2, VOXQ_ROPE_YARN = 3, VOXQ_ROPE_LONG = 4 };
+typedef struct {
+    int32_t n_pos, rot_dim, scaling;
+    double theta, factor;
+    double beta_fast, beta_slow;   /* VOXQ_ROPE_YARN; 0 -> 32 and 1 */
+    double attn_factor;            /* 0 -> 1 */
+    int32_t original_len;          /* VOXQ_ROPE_YARN */
+    const double* long_factors;    /* VOXQ_ROPE_LONG: host [rot_dim / 2], read before the call returns; rot_dim <= 256 */
+    float* out;                    /* [n_pos][rot_dim / 2][2] */
+} voxq_rope_table;
+VOXQ_API VoxCPMError voxq_rope_freqs(const voxq_rope_table* d, void* stream);
+
+/* Rotates the new tokens' queries and keys and writes keys and values into a
+ * paged cache, in one pass.  For token t at position p = positions[t] and
+ * pair i < rot_dim / 2 with (c, s) = freqs[p][i]:
+ *   (x0, x1) -> (x0 c - x1 s, x0 s + x1 c), where (x0, x1) are elements
+ *   (i, i + rot_dim / 2) of the head, or (2 i, 2 i + 1) when interleaved;
+ * elements from rot_dim on pass through.  q_out gets the rotated queries
+ * (NULL: no queries); row slots[t] = page * page_size + offset of the caches
+ * gets the rotated key and the value; a slot < 0 or past the pool writes
+ * neither (padding tokens).  q, k, v are in_dtype; q_out and the caches are
+ * cache_dtype: the same type, or any of the three for fp32 inputs (rounded
+ * once, to nearest even).  q_out may alias q when the types match.  16-byte
+ * rows for every tensor; head_dim a multiple of 8 up to 256, rot_dim even. */
+typedef struct {
+    const void *q, *k, *v;                /* [tokens][heads or kv_heads][head_dim] */
+    int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
+    void* q_out;
+    int64_t qo_stride, qo_head_stride;
+    void *cache_k, *cache_v;              /* [pages][page_size][kv_heads][head_dim], the same strides for both */
+    int64_t page_stride, row_stride, head_stride;
+    const float* freqs;                   /* [n_pos][rot_dim / 2][2]; NULL: no rotation (rot_dim 0) */
+    const int32_t* positions;             /* [tokens], clamped to [0, n_pos) */
+    const int64_t* slots;                 /* [tokens] */
+    int32_t tokens, heads, kv_heads, head_dim, rot_dim, interleaved, n_pos;
+    int32_t pages, page_size;
+    int32_t in_dtype, cache_dtype;
+} voxq_rope;
+VOXQ_API VoxCPMError voxq_rope_append(const voxq_rope* d, void* stream);
+
+/* Attention of each sequence's new tokens over its pages: for row i of the n
+ * rows of a sequence with kv_len cached positions (its new ones included)
+ *   out_i = sum_j softmax_j(scale q_i . k_j) v_j over j < kv_len and, when
+ *   causal, j <= kv_len - n + i;
+ * a row that sees no key gives zeros.  Query head h reads kv head
+ * h / (heads / kv_heads).  Position j of sequence s is row j % page_size of
+ * page block_table[s][j / page_size] (entries outside [0, pages) read page
+ * 0); page_size is any number.  Cache rows at or past kv_len may hold anything, NaN
+ * included.  q, k, v are one type; out is that type or VOXQ_F32.  In the 16-bit types the products take
+ * 16-bit operands with fp32 accumulation.  max_q and max_kv are upper bounds
+ * of the sequences' new tokens and lengths (they choose the kernel and size
+ * its grid; kv_len is clamped to max_kv).  16-byte rows; head_dim a multiple
+ * of 8 up to 256; heads / kv_heads any whole number.
+ * voxq_paged_attention_workspace gives the bytes of `workspace` (256-byte
+ * aligned, contents irrelevant, in use until the call's work is done; 0: none
+ * needed), from the integer fields alone. */
+typedef struct {
+    const void* q;                        /* [total_q][heads][head_dim] */
+    int64_t q_stride, q_head_stride;
+    void* out;
+    int64_t o_stride, o_head_stride;
+    const void *k, *v;                    /* [pages][page_size][kv_heads][head_dim], the same strides for both */
+    int64_t page_stride, row_stride, head_stride;
+    const int32_t* block_table;           /* [batch][table_stride] */
+    int64_t table_stride;
+    const int32_t *cu_q, *kv_len;         /* [batch + 1], [batch] */
+    int32_t batch, heads, kv_heads, head_dim, pages, page_size;
+    int32_t total_q, max_q, max_kv;
+    int32_t dtype, out_dtype, causal;
+    float scale;                          /* 0: 1 / sqrt(head_dim) */
+    void* workspace;
+    size_t workspace_bytes;
+} voxq_paged_attn;
+VOXQ_API size_t voxq_paged_attention_workspace(const voxq_paged_attn* d);
+VOXQ_API VoxCPMError voxq_paged_attention(const voxq_paged_attn* d, void* stream);
+
+/* Low-rank adapters of many requests beside a shared projection:
+ *   out[m] = base[m] + scale[w] * (x[m] A[w]^T) B[w]^T
+ * for the rows m of request s with w = adapter[s] in [0, adapters); rows of a
+ * request without one (w outside the range) get base[m].  A is [adapters]
+ * [rank][K], B is [adapters][N][rank]; ranks (NULL: all `rank`) gives each
+ * adapter's own rank, at most `rank`: columns from there on are not used.
+ * base NULL counts as zeros; out may be base.  x, base and out are one type;
+ * A and B are that type, or any of the three for fp32 x.  16-byte rows; K, N
+ * and rank multiples of 8, rank <= 128. */
+typedef struct {
+    const void* x;
+    int64_t ldx;
+    const void* base;
+    int64_t ldb;
+    void* out;
+    int64_t ldo;
+    const void *a, *b;
+    const int32_t *cu, *adapter, *ranks;  /* [batch + 1], [batch], [adapters] or NULL */
+    const float* scale;                   /* [adapters] */
+    int32_t rows, batch, K, N, rank, adapters;
+    int32_t dtype, w_dtype;
+} voxq_lora;
+VOXQ_API VoxCPMError voxq_lora_forward(const voxq_lora* d, void* stream);
+
+/* The norms around a block, its gate and its residual scale in one pass:
+ *   z = y, or RMSNorm(y) * w_post when w_post is given
+ *   h = x + alpha * gate[g(m)] * z      (gate NULL: no gate)
+ *   n = RMSNorm(h) * w_pre              (n_out NULL: no second norm)
+ * RMSNorm(v) = v / sqrt(mean(v^2) + eps), in fp32 on the unrounded h.  g(m) is
+ * gate_index[m] clamped to [0, gate_rows), or, with gate_index NULL, m when
+ * gate_rows == rows and 0 when gate_rows == 1.  h_out may be x or y, n_out may be y or x (not both one buffer).
+ * y, x, gate, h_out and n_out are one type, the norm weights
+ * fp32.  Any D from 1 to 16384 and any alignment (16-byte rows take wide
+ * loads). */
+typedef struct {
+    const void *y, *x, *gate;
+    int64_t ldy, ldx, ldg;
+    const float *w_post, *w_pre;
+    const int32_t* gate_index;
+    void *h_out, *n_out;
+    int64_t ldh, ldn;
+    int32_t rows, D, gate_rows, dtype;
+    float alpha, eps;
+} voxq_norm;
+VOXQ_API VoxCPMError voxq_norm_residual(const voxq_norm* d, void* stream);
 
 /* ---- quantize.py weight containers (VXCPM2) ---------------------------
  * Reads the container written by the reference's quantizer

@@ -21,6 +21,7 @@ PKG = os.path.dirname(HERE)
 LIB_PATH = os.path.join(PKG, "libvoxq.so")
 
 F32, F16, Q4, Q8 = 0, 1, 2, 3  # scripts/quantize.py:28 QUANT_TYPES
+BF16 = 4  # element type of the batched-step operators
 BLOCK = 32
 MAX_BATCH = 192
 
@@ -140,6 +141,46 @@ class LocEncDesc(C.Structure):
                 ("output_norm", C.POINTER(RmsNormDesc)), ("d_model", C.c_int), ("patch_size", C.c_int)]
 
 
+def _fields(spec: str):
+    """ctypes fields from "type: names" lines (p pointer, l int64, i int32, f float, d double, z size_t)."""
+    types = {"p": C.c_void_p, "l": C.c_int64, "i": C.c_int32, "f": C.c_float, "d": C.c_double, "z": C.c_size_t}
+    return [(n, types[part.split(":")[0].strip()]) for part in spec.split(";") for n in part.split(":")[1].split()]
+
+
+class RopeTableDesc(C.Structure):
+    """voxq_rope_table (include/voxq.h)."""
+    _fields_ = _fields("i: n_pos rot_dim scaling; d: theta factor beta_fast beta_slow attn_factor; i: original_len; "
+                       "p: long_factors out")
+
+
+class RopeDesc(C.Structure):
+    """voxq_rope (include/voxq.h)."""
+    _fields_ = _fields("p: q k v; l: q_stride q_head_stride k_stride k_head_stride v_stride v_head_stride; p: q_out; "
+                       "l: qo_stride qo_head_stride; p: cache_k cache_v; l: page_stride row_stride head_stride; "
+                       "p: freqs positions slots; i: tokens heads kv_heads head_dim rot_dim interleaved n_pos pages "
+                       "page_size in_dtype cache_dtype")
+
+
+class PagedAttnDesc(C.Structure):
+    """voxq_paged_attn (include/voxq.h)."""
+    _fields_ = _fields("p: q; l: q_stride q_head_stride; p: out; l: o_stride o_head_stride; p: k v; "
+                       "l: page_stride row_stride head_stride; p: block_table; l: table_stride; p: cu_q kv_len; "
+                       "i: batch heads kv_heads head_dim pages page_size total_q max_q max_kv dtype out_dtype causal; "
+                       "f: scale; p: workspace; z: workspace_bytes")
+
+
+class LoraDesc(C.Structure):
+    """voxq_lora (include/voxq.h)."""
+    _fields_ = _fields("p: x; l: ldx; p: base; l: ldb; p: out; l: ldo; p: a b cu adapter ranks scale; "
+                       "i: rows batch K N rank adapters dtype w_dtype")
+
+
+class NormDesc(C.Structure):
+    """voxq_norm (include/voxq.h)."""
+    _fields_ = _fields("p: y x gate; l: ldy ldx ldg; p: w_post w_pre gate_index h_out n_out; l: ldh ldn; "
+                       "i: rows D gate_rows dtype; f: alpha eps")
+
+
 _vp, _sz, _i, _i64 = C.c_void_p, C.c_size_t, C.c_int, C.c_int64
 _TP = C.POINTER(Tensor)
 SIGNATURES = {
@@ -176,6 +217,12 @@ SIGNATURES = {
     "voxq_block_cache_clear": ([], None),
     "voxq_locdit_sample": ([_vp, _TP, _TP, _i, C.c_float, _TP, _TP], _i),
     "voxq_locenc_forward": ([_vp, _TP, _TP], _i),
+    "voxq_rope_freqs": ([C.POINTER(RopeTableDesc), _vp], _i),
+    "voxq_rope_append": ([C.POINTER(RopeDesc), _vp], _i),
+    "voxq_paged_attention_workspace": ([C.POINTER(PagedAttnDesc)], _sz),
+    "voxq_paged_attention": ([C.POINTER(PagedAttnDesc), _vp], _i),
+    "voxq_lora_forward": ([C.POINTER(LoraDesc), _vp], _i),
+    "voxq_norm_residual": ([C.POINTER(NormDesc), _vp], _i),
     "voxq_vxcpm2_open": ([C.c_char_p, C.POINTER(_vp)], _i),
     "voxq_vxcpm2_close": ([_vp], None),
     "voxq_vxcpm2_info": ([_vp, C.POINTER(Vxcpm2Header), C.POINTER(_i)], _i),
@@ -368,6 +415,22 @@ def set_device(d: int) -> None:
 
 def version() -> str:
     return lib().voxq_version().decode()
+
+
+# ---------------------------------------------------------------------------
+# A decoder step over many utterances (voxq/batched.py, loaded on first use:
+# it needs torch, which this module imports only inside its functions)
+# ---------------------------------------------------------------------------
+
+_BATCHED = ("rope_freqs", "rope_append", "paged_attention", "lora", "norm_residual")
+
+
+def __getattr__(name):
+    if name in _BATCHED:
+        from . import batched
+        globals().update({n: getattr(batched, n) for n in _BATCHED})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 # ---------------------------------------------------------------------------

@@ -6,6 +6,7 @@
 #include <cuda_bf16.h>
 
 #include "voxq_common.cuh"
+#include "voxq_internal.h"
 
 namespace voxq {
 
@@ -31,6 +32,24 @@ template <>
 __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
 template <>
 __device__ __forceinline__ bf16 from_f<bf16>(float x) { return __float2bfloat16_rn(x); }
+
+// Launches with programmatic stream serialization (see pdl_enabled): the
+// kernel may start while its predecessor drains and must execute pdl_wait()
+// before its first access to global memory.
+template <typename... P, typename... A>
+inline cudaError_t launch_pdl(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, P(args)...);
+}
 
 // Calls f with a value of the element type that `dtype` names.
 template <typename F>

@@ -5,59 +5,179 @@
 
 namespace voxq {
 
-constexpr int kNormThreads = 256;
 constexpr int kNormMaxD = 16384;
 
-__device__ __forceinline__ float block_sum(float v, float* red) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float s = 0.0f;
-    for (int w = 0; w < kNormThreads / 32; w++) s += red[w];
-    return s;
+// V contiguous elements in one access (16 bytes, or one element where a row
+// or its width is not 16-byte aligned).
+template <typename T, int V>
+struct Vec {
+    T e[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
+    Vec<T, V> r;
+    if constexpr (V > 1) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        memcpy(&r, &v, 16);
+    } else {
+        r.e[0] = *p;
+    }
+    return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& r) {
+    if constexpr (V > 1) {
+        uint4 v;
+        memcpy(&v, &r, 16);
+        *reinterpret_cast<uint4*>(p) = v;
+    } else {
+        *p = r.e[0];
+    }
 }
 
-// One row per CTA, held in registers between the passes.
-template <typename T>
-__global__ void __launch_bounds__(kNormThreads) norm_residual_kernel(const voxq_norm d) {
-    __shared__ float red[kNormThreads / 32];
-    const int m = blockIdx.x;
+// The norm weights go through the read-only path, so that their loads may be
+// issued ahead of the stores of h, which the compiler cannot tell apart.
+template <int V>
+__device__ __forceinline__ void load_weights(float (&w)[V], const float* p) {
+    if constexpr (V == 1) {
+        w[0] = __ldg(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 4; i++) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(p) + i);
+            w[4 * i] = v.x;
+            w[4 * i + 1] = v.y;
+            w[4 * i + 2] = v.z;
+            w[4 * i + 3] = v.w;
+        }
+    }
+}
+
+// Sum over the WR warps of a row, the same value in every thread.
+template <int WR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if constexpr (WR > 1) {
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WR; w++) v += red[w];
+    }
+    return v;
+}
+
+// h = x + alpha g z and n = RMSNorm(h) w_pre, z = y or RMSNorm(y) w_post.
+// 2 reads and 2 writes per element and a few flops: bound by HBM for many
+// rows, by the latency of one load and two reductions for a few.  WR warps
+// hold a whole row in registers, PER vectors of V elements a thread, so the
+// second norm needs no second read; all of a row's loads are issued before the
+// first reduction, and with one warp per row no block barrier is needed.
+// h stays fp32 from its sum to the norm.
+template <typename T, int V, int WR, int PER>
+__global__ void __launch_bounds__(WR == 1 ? 128 : 32 * WR) norm_residual_kernel(const __grid_constant__ voxq_norm d) {
+    __shared__ float red[2][WR];
+    const int m = WR == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    if (WR == 1 && m >= d.rows) return;
+    const int tid = WR == 1 ? threadIdx.x & 31 : threadIdx.x;
     const T* y = (const T*)d.y + m * d.ldy;
     const T* x = (const T*)d.x + m * d.ldx;
+    pdl_wait();
+    pdl_launch_dependents();
+    Vec<T, V> yv[PER], xv[PER], gv[PER];
     const T* g = nullptr;
-    if (d.gate) {
-        const int r = d.gate_index ? min(max(d.gate_index[m], 0), d.gate_rows - 1) : d.gate_rows == 1 ? 0 : m;
-        g = (const T*)d.gate + r * d.ldg;
+    if (d.gate) g = (const T*)d.gate + (d.gate_index ? min(max(__ldg(d.gate_index + m), 0), d.gate_rows - 1) : d.gate_rows == 1 ? 0 : m) * d.ldg;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        const int i = (tid + j * 32 * WR) * V;
+        if (i < d.D) {
+            yv[j] = load_vec<T, V>(y + i);
+            xv[j] = load_vec<T, V>(x + i);
+        }
     }
+    if (g)
+#pragma unroll
+        for (int j = 0; j < PER; j++)
+            if ((tid + j * 32 * WR) * V < d.D) gv[j] = load_vec<T, V>(g + (tid + j * 32 * WR) * V);
     float inv = 1.0f;
     if (d.w_post) {
         float s = 0.0f;
-        for (int i = threadIdx.x; i < d.D; i += kNormThreads) s += to_f(y[i]) * to_f(y[i]);
-        inv = rsqrtf(block_sum(s, red) / d.D + d.eps);
+#pragma unroll
+        for (int j = 0; j < PER; j++)
+            if ((tid + j * 32 * WR) * V < d.D)
+#pragma unroll
+                for (int e = 0; e < V; e++) s = fmaf(to_f(yv[j].e[e]), to_f(yv[j].e[e]), s);
+        inv = rsqrtf(row_sum<WR>(s, red[0]) / d.D + d.eps);
     }
-    constexpr int PER = kNormMaxD / kNormThreads;
-    float hr[PER];
-    float s = 0.0f;
+    float h[PER][V], s = 0.0f;
 #pragma unroll
     for (int j = 0; j < PER; j++) {
-        const int i = threadIdx.x + j * kNormThreads;
-        hr[j] = 0.0f;
+        const int i = (tid + j * 32 * WR) * V;
         if (i >= d.D) continue;
-        float z = to_f(y[i]);
-        if (d.w_post) z = z * inv * d.w_post[i];
-        if (g) z *= to_f(g[i]);
-        hr[j] = to_f(x[i]) + d.alpha * z;
-        s += hr[j] * hr[j];
+        float w[V];
+        if (d.w_post) load_weights<V>(w, d.w_post + i);
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            float z = to_f(yv[j].e[e]);
+            if (d.w_post) z = z * inv * w[e];
+            if (g) z *= to_f(gv[j].e[e]);
+            h[j][e] = fmaf(d.alpha, z, to_f(xv[j].e[e]));
+            s = fmaf(h[j][e], h[j][e], s);
+        }
     }
-    inv = d.n_out ? rsqrtf(block_sum(s, red) / d.D + d.eps) : 0.0f;
+    if (d.h_out)
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int i = (tid + j * 32 * WR) * V;
+            if (i >= d.D) continue;
+            Vec<T, V> hv;
+#pragma unroll
+            for (int e = 0; e < V; e++) hv.e[e] = from_f<T>(h[j][e]);
+            store_vec<T, V>((T*)d.h_out + m * d.ldh + i, hv);
+        }
+    if (!d.n_out) return;
+    inv = rsqrtf(row_sum<WR>(s, red[1]) / d.D + d.eps);
 #pragma unroll
     for (int j = 0; j < PER; j++) {
-        const int i = threadIdx.x + j * kNormThreads;
+        const int i = (tid + j * 32 * WR) * V;
         if (i >= d.D) continue;
-        if (d.h_out) ((T*)d.h_out + m * d.ldh)[i] = from_f<T>(hr[j]);
-        if (d.n_out) ((T*)d.n_out + m * d.ldn)[i] = from_f<T>(hr[j] * inv * d.w_pre[i]);
+        float w[V];
+        load_weights<V>(w, d.w_pre + i);
+        Vec<T, V> nv;
+#pragma unroll
+        for (int e = 0; e < V; e++) nv.e[e] = from_f<T>(h[j][e] * inv * w[e]);
+        store_vec<T, V>((T*)d.n_out + m * d.ldn + i, nv);
+    }
+}
+
+template <typename T, int V, int WR, int PER>
+static cudaError_t norm_launch(const voxq_norm& d, cudaStream_t st) {
+    const int blocks = WR == 1 ? (d.rows + 3) / 4 : d.rows;
+    return launch_pdl(norm_residual_kernel<T, V, WR, PER>, dim3(blocks), dim3(WR == 1 ? 128 : 32 * WR), 0, st, d);
+}
+
+// Warps per row: as few as hold it in 8 vectors a thread when there are rows
+// enough to fill the GPU (no block barrier, most bytes in flight per thread),
+// else as many as leave 2 (shorter chains per thread).
+template <typename T>
+static cudaError_t norm_dispatch(const voxq_norm& d, bool wide, cudaStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    if (!wide)  // odd widths and alignments, one element per access
+        return d.D <= 1024 ? norm_launch<T, 1, 4, 8>(d, st) : norm_launch<T, 1, 16, 32>(d, st);
+    const int nv = d.D / V;
+    const bool few = d.rows < 8 * device_sm_count();
+    if (nv <= (few ? 64 : 256)) {
+        if (nv <= 64) return norm_launch<T, V, 1, 2>(d, st);
+        else if (nv <= 128) return norm_launch<T, V, 1, 4>(d, st);
+        else return norm_launch<T, V, 1, 8>(d, st);
+    } else if (nv <= (few ? 256 : 1024)) {
+        if (nv <= 256) return norm_launch<T, V, 4, 2>(d, st);
+        else return norm_launch<T, V, 4, 8>(d, st);
+    } else if (nv <= 1024) {
+        return norm_launch<T, V, 16, 2>(d, st);
+    } else {
+        return norm_launch<T, V, 16, 8>(d, st);
     }
 }
 
@@ -73,9 +193,10 @@ extern "C" VoxCPMError voxq_norm_residual(const voxq_norm* d, void* stream) {
     if (!d->y || !d->x || (!d->h_out && !d->n_out) || (d->n_out && !d->w_pre)) return VOXCPM_ERR_INTERNAL;
     if (d->gate && (d->gate_rows == 0 || (!d->gate_index && d->gate_rows != 1 && d->gate_rows != d->rows)))
         return VOXCPM_ERR_SHAPE_MISMATCH;
-    with_elem(d->dtype, [&](auto x) {
-        norm_residual_kernel<decltype(x)><<<d->rows, kNormThreads, 0, (cudaStream_t)stream>>>(*d);
-    });
-    VOXQ_CUDA_TRY(cudaGetLastError());
+    const int dt = d->dtype;
+    const bool wide = d->D % (16 / elem_bytes(dt)) == 0 && rows16(d->y, d->ldy, dt) && rows16(d->x, d->ldx, dt) &&
+                      (!d->gate || rows16(d->gate, d->ldg, dt)) && (!d->h_out || rows16(d->h_out, d->ldh, dt)) &&
+                      (!d->n_out || rows16(d->n_out, d->ldn, dt)) && rows16(d->w_post, 0, VOXQ_F32) && rows16(d->w_pre, 0, VOXQ_F32);
+    VOXQ_CUDA_TRY(with_elem(dt, [&](auto x) { return norm_dispatch<decltype(x)>(*d, wide, (cudaStream_t)stream); }));
     return VOXCPM_SUCCESS;
 }

@@ -2,10 +2,15 @@
 // their write into a paged KV cache.
 #include <math.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "voxq_batch.cuh"
 #include "voxq_internal.h"
 
 namespace voxq {
+
+constexpr int kRopeThreads = 256;
 
 struct RopeFreqs {
     double inv[128];  // angle per position of each pair
@@ -25,37 +30,131 @@ __global__ void __launch_bounds__(256) rope_table_kernel(const __grid_constant__
     }
 }
 
-// One element pair per thread.
-template <typename T, typename C>
-__global__ void __launch_bounds__(128) rope_append_kernel(const voxq_rope d) {
-    const int t = blockIdx.x, slot_h = blockIdx.y;
-    const int half = d.rot_dim / 2, H = d.heads, KVH = d.kv_heads;
-    const T* src;
-    C* dst;
-    bool turn = d.freqs != nullptr;
-    if (slot_h < H) {
-        src = (const T*)d.q + t * d.q_stride + slot_h * d.q_head_stride;
-        dst = (C*)d.q_out + t * d.qo_stride + slot_h * d.qo_head_stride;
+// N contiguous elements as fp32 and back, in 16-byte (or, for runs of four
+// 16-bit elements, 8-byte) accesses; N = 1 for odd rotary halves.
+template <int N, typename T>
+__device__ __forceinline__ void load_run(float (&x)[N], const T* p) {
+    if constexpr (N == 1) {
+        x[0] = to_f(p[0]);
     } else {
-        const int64_t slot = d.slots[t];
-        if (slot < 0 || slot >= (int64_t)d.pages * d.page_size) return;
-        const bool key = slot_h < H + KVH;
-        const int h = key ? slot_h - H : slot_h - H - KVH;
-        src = key ? (const T*)d.k + t * d.k_stride + h * d.k_head_stride : (const T*)d.v + t * d.v_stride + h * d.v_head_stride;
-        dst = (C*)(key ? d.cache_k : d.cache_v) + (slot / d.page_size) * d.page_stride +
-              (slot % d.page_size) * d.row_stride + h * d.head_stride;
-        turn = turn && key;
+        constexpr int W = N * sizeof(T) >= 16 ? 16 : 8;  // bytes per access
+        using V = typename std::conditional<W == 16, uint4, uint2>::type;
+        constexpr int E = W / sizeof(T);
+#pragma unroll
+        for (int j = 0; j < N / E; j++) {
+            const V v = reinterpret_cast<const V*>(p)[j];
+            T e[E];
+            memcpy(e, &v, W);
+#pragma unroll
+            for (int i = 0; i < E; i++) x[j * E + i] = to_f(e[i]);
+        }
     }
-    const int rot = turn ? d.rot_dim : 0;
-    const float* f = d.freqs;
-    if (turn) f += (int64_t)min(max(d.positions[t], 0), d.n_pos - 1) * d.rot_dim;
-    for (int i = threadIdx.x; i < rot / 2; i += 128) {
-        const int i0 = d.interleaved ? 2 * i : i, i1 = d.interleaved ? 2 * i + 1 : i + half;
-        const float x0 = to_f(src[i0]), x1 = to_f(src[i1]), c = f[2 * i], s = f[2 * i + 1];
-        dst[i0] = from_f<C>(x0 * c - x1 * s);
-        dst[i1] = from_f<C>(x0 * s + x1 * c);
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_run(T* p, const float (&x)[N]) {
+    if constexpr (N == 1) {
+        p[0] = from_f<T>(x[0]);
+    } else {
+        constexpr int W = N * sizeof(T) >= 16 ? 16 : 8;
+        using V = typename std::conditional<W == 16, uint4, uint2>::type;
+        constexpr int E = W / sizeof(T);
+#pragma unroll
+        for (int j = 0; j < N / E; j++) {
+            T e[E];
+#pragma unroll
+            for (int i = 0; i < E; i++) e[i] = from_f<T>(x[j * E + i]);
+            V v;
+            memcpy(&v, e, W);
+            reinterpret_cast<V*>(p)[j] = v;
+        }
     }
-    for (int i = rot + threadIdx.x; i < d.head_dim; i += 128) dst[i] = from_f<C>(to_f(src[i]));
+}
+
+// One pass over q, k and v, bound by HBM for prompts and by the latency of its
+// one chain (position -> table row -> store) for a step.  A CTA takes one
+// token; thread (x, y) takes CH pairs of head y, y + blockDim.y, ...: two runs
+// of CH elements half a rotary width apart, or one of 2 CH when interleaved,
+// so every access is a full vector.  The elements behind rot_dim are items of
+// 2 CH elements as well.  The inputs do not depend on the position, so their
+// loads are in flight together with it.
+template <typename T, typename C, int CH, bool INTER>
+__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const __grid_constant__ voxq_rope d) {
+    const int t = blockIdx.x, item = threadIdx.x;
+    const int half = d.rot_dim / 2, H = d.heads, heads = H + 2 * d.kv_heads;
+    const int turning = half / CH;  // items that rotate
+    const bool turn = item < turning;
+    const int i0 = !turn ? d.rot_dim + (item - turning) * 2 * CH : INTER ? item * 2 * CH : item * CH;
+    const int i1 = turn && !INTER ? i0 + half : i0 + CH;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int64_t slot = d.kv_heads ? d.slots[t] : -1;
+    const int p = d.freqs ? min(max(d.positions[t], 0), d.n_pos - 1) : 0;
+    float c[CH], s[CH];
+#pragma unroll
+    for (int j = 0; j < CH; j++) {
+        c[j] = 1.0f;
+        s[j] = 0.0f;
+    }
+    if (turn) {
+        const float2* f = reinterpret_cast<const float2*>(d.freqs) + (int64_t)p * half + item * CH;
+#pragma unroll
+        for (int j = 0; j < CH; j++) {
+            const float2 v = __ldg(f + j);
+            c[j] = v.x;
+            s[j] = v.y;
+        }
+    }
+    const bool live = slot >= 0 && slot < (int64_t)d.pages * d.page_size;
+    const uint32_t row = live ? (uint32_t)slot : 0u, page = d.page_size ? row / (uint32_t)d.page_size : 0u;
+    const int64_t place = page * d.page_stride + (row - page * d.page_size) * d.row_stride;
+    for (int h = threadIdx.y; h < heads; h += blockDim.y) {
+        const T* src;
+        C* dst;
+        bool rot = turn;
+        if (h < H) {
+            src = (const T*)d.q + t * d.q_stride + h * d.q_head_stride;
+            dst = (C*)d.q_out + t * d.qo_stride + h * d.qo_head_stride;
+        } else {
+            const int kh = h - H < d.kv_heads ? h - H : h - H - d.kv_heads;
+            if (!live) continue;
+            rot = turn && h - H < d.kv_heads;
+            src = h - H < d.kv_heads ? (const T*)d.k + t * d.k_stride + kh * d.k_head_stride
+                                     : (const T*)d.v + t * d.v_stride + kh * d.v_head_stride;
+            dst = (C*)(h - H < d.kv_heads ? d.cache_k : d.cache_v) + place + kh * d.head_stride;
+        }
+        float a[CH], b[CH];
+        load_run<CH>(a, src + i0);
+        load_run<CH>(b, src + i1);
+        if (rot) {
+            if (INTER) {  // a holds pairs 0 .. CH/2 - 1 side by side, b the rest
+#pragma unroll
+                for (int j = 0; j < CH; j++) {
+                    float& x0 = 2 * j < CH ? a[2 * j % CH] : b[2 * j % CH];
+                    float& x1 = 2 * j + 1 < CH ? a[(2 * j + 1) % CH] : b[(2 * j + 1) % CH];
+                    const float y0 = x0 * c[j] - x1 * s[j], y1 = x0 * s[j] + x1 * c[j];
+                    x0 = y0;
+                    x1 = y1;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < CH; j++) {
+                    const float y0 = a[j] * c[j] - b[j] * s[j], y1 = a[j] * s[j] + b[j] * c[j];
+                    a[j] = y0;
+                    b[j] = y1;
+                }
+            }
+        }
+        store_run<CH>(dst + i0, a);
+        store_run<CH>(dst + i1, b);
+    }
+}
+
+template <typename T, typename C, int CH>
+static cudaError_t rope_launch(const voxq_rope& p, cudaStream_t st) {
+    const int items = p.head_dim / (2 * CH), heads = p.heads + 2 * p.kv_heads;
+    const dim3 block(items, std::max(1, std::min(heads, kRopeThreads / items)));
+    return launch_pdl(p.interleaved ? rope_append_kernel<T, C, CH, true> : rope_append_kernel<T, C, CH, false>,
+                      dim3(p.tokens), block, 0, st, p);
 }
 
 }  // namespace voxq
@@ -113,6 +212,7 @@ extern "C" VoxCPMError voxq_rope_append(const voxq_rope* d, void* stream) {
     if (d->tokens < 0 || d->heads < 0 || d->kv_heads < 0 || d->head_dim < 0 || d->rot_dim < 0 || d->pages < 0 ||
         d->page_size < 0 || d->rot_dim > d->head_dim || d->rot_dim % 2)
         return VOXCPM_ERR_SHAPE_MISMATCH;
+    if ((int64_t)d->pages * d->page_size > INT32_MAX) return VOXCPM_ERR_UNSUPPORTED;
     if (!elem_ok(d->in_dtype) || !elem_ok(d->cache_dtype) || (d->in_dtype != VOXQ_F32 && d->in_dtype != d->cache_dtype) ||
         d->head_dim % 8 || d->head_dim > 256)
         return VOXCPM_ERR_UNSUPPORTED;
@@ -136,11 +236,22 @@ extern "C" VoxCPMError voxq_rope_append(const voxq_rope* d, void* stream) {
     p.heads = heads;
     if (!turn) p.freqs = nullptr;
     if (!store) p.kv_heads = 0;
-    const dim3 grid(p.tokens, p.heads + 2 * p.kv_heads);
+    if (!turn) p.rot_dim = 0;
     cudaStream_t st = (cudaStream_t)stream;
+    // the widest run that divides both the rotary half and the rest of the head
+    const int half = p.rot_dim / 2, rest = p.head_dim - p.rot_dim;
+    cudaError_t e = cudaSuccess;
     with_elem(it, [&](auto x) {
-        with_elem(ct, [&](auto y) { rope_append_kernel<decltype(x), decltype(y)><<<grid, 128, 0, st>>>(p); });
+        with_elem(ct, [&](auto y) {
+            using T = decltype(x);
+            using C = decltype(y);
+            if constexpr (std::is_same<T, float>::value || std::is_same<T, C>::value) {
+                if (half % 8 == 0 && rest % 16 == 0) e = rope_launch<T, C, 8>(p, st);
+                else if (half % 4 == 0 && rest % 8 == 0) e = rope_launch<T, C, 4>(p, st);
+                else e = rope_launch<T, C, 1>(p, st);
+            }
+        });
     });
-    VOXQ_CUDA_TRY(cudaGetLastError());
+    VOXQ_CUDA_TRY(e);
     return VOXCPM_SUCCESS;
 }

@@ -598,7 +598,8 @@ VOXQ_API VoxCPMError voxq_paged_attention(const voxq_paged_attn* d, void* stream
  * adapter's own rank, at most `rank`: columns from there on are not used.
  * base NULL counts as zeros; out may be base.  x, base and out are one type;
  * A and B are that type, or any of the three for fp32 x.  16-byte rows; K, N
- * and rank multiples of 8, rank <= 128. */
+ * and rank multiples of 8, rank <= 128.  cu[batch] is rows: a row that no request owns is not
+ * written.  In fp16, scale (x A^T) must lie in fp16's range. */
 typedef struct {
     const void* x;
     int64_t ldx;

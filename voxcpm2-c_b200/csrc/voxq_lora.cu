@@ -1,48 +1,391 @@
 // voxq_lora.cu -- low-rank adapters of many requests beside a shared projection.
+#include <mutex>
+#include <type_traits>
+
 #include "voxq_batch.cuh"
 #include "voxq_internal.h"
 
 namespace voxq {
 
-constexpr int kLoraThreads = 256;
+constexpr int kLoraThreads = 128;
+constexpr int kLoraWarps = kLoraThreads / 32;
 constexpr int kLoraMaxRank = 128;
 
-// The request that owns row m: the last s with cu[s] <= m.
-__device__ __forceinline__ int owner(const int32_t* __restrict__ cu, int batch, int m) {
-    int lo = 0, hi = batch - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (cu[mid] <= m) lo = mid;
-        else hi = mid - 1;
+template <typename T>
+constexpr bool is_f32 = std::is_same<T, float>::value;
+
+// Shape of the kernel for x of type T, weights of type W and TM rows a tile.
+template <typename T, typename W, int TM>
+struct LoraShape {
+    static constexpr int WM = TM / 16;                // warps along the rows
+    static constexpr int WK = kLoraWarps / WM;        // warps along K (first product) or the columns (second)
+    static constexpr int KB = is_f32<W> || (is_f32<T> && TM == 64) ? 64 : 128;  // K per stage (two fit in shared memory)
+    static constexpr int NB = TM == 64 ? 64 : 128;    // output columns per step
+    static constexpr int NW = NB / WK;                // of a warp
+    static constexpr int XP = KB + 16 / sizeof(T);    // shared pitches: 16 bytes more than a row, so that the 8 rows
+    static constexpr int AP = KB + 16 / sizeof(W);    // of a fragment load lie in different banks
+    static constexpr int OP = NW + 4;
+    int Rp, stage, hp, bp;                            // rank in steps of 16; bytes of a stage; pitches of h and B
+    int o_hpart, o_hs, o_b0, o_b1, o_out, bytes;      // byte offsets
+    __host__ __device__ explicit LoraShape(int rank) {
+        Rp = (rank + 15) / 16 * 16;
+        stage = TM * XP * (int)sizeof(T) + Rp * AP * (int)sizeof(W);
+        hp = Rp + 8;
+        bp = Rp + 16 / (int)sizeof(W);
+        // the stages are free once the first product is done: the second
+        // buffer of B and the output staging live there
+        const int bbytes = NB * bp * (int)sizeof(W), obytes = kLoraWarps * 16 * OP * 4;
+        o_b1 = 0;
+        o_out = bbytes;
+        const int low = 2 * stage > bbytes + obytes ? 2 * stage : bbytes + obytes;
+        o_hpart = (low + 15) / 16 * 16;
+        o_hs = o_hpart + WK * TM * hp * 4;
+        o_b0 = o_hs + TM * hp * 4;  // fp32, or two 16-bit parts
+        bytes = o_b0 + bbytes;
     }
-    return lo;
+};
+
+// 16 bytes to shared memory, zeros when !ok (the source is then not read).
+__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
 
-// One row per CTA: h = scale A x in shared memory (a warp per rank), then every
-// thread its output columns.
-template <typename T, typename W>
-__global__ void __launch_bounds__(kLoraThreads) lora_kernel(const voxq_lora d) {
-    __shared__ float h[kLoraMaxRank];
-    const int m = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int w = d.batch ? d.adapter[owner(d.cu, d.batch, m)] : -1;
-    const bool on = w >= 0 && w < d.adapters;
-    const int rank = !on ? 0 : d.ranks ? min(max(d.ranks[w], 0), d.rank) : d.rank;
-    const T* x = (const T*)d.x + m * d.ldx;
-    for (int r = warp; r < rank; r += kLoraThreads / 32) {
-        const W* a = (const W*)d.a + ((int64_t)w * d.rank + r) * d.K;
-        float s = 0.0f;
-        for (int k = lane; k < d.K; k += 32) s = fmaf(to_f(x[k]), to_f(a[k]), s);
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// x as a sum of two TF32 values: what is left out is below 2^-22 of it.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    const float r = x - __uint_as_float(hi);
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(r));
+}
+
+// d[i] += a b[i]^T over 16 of the inner dimension, the 16 x 16 a at `as` and NBLK 8-row blocks of b at `bs`, both in
+// shared memory with the inner dimension contiguous.  16-bit: one MMA per block (and one more for a's low part at
+// as_lo).  fp32: TF32 MMAs on a's high and low parts and, for fp32 weights, on b's; a 16-bit weight is a TF32 value.
+template <typename T, typename W, int NBLK, bool LOW>
+__device__ __forceinline__ void mul_16(float (*d)[4], const T* as, const T* as_lo, int ap, const W* bs, int bp, int blocks) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    if constexpr (!is_f32<T>) {
+        uint32_t a[4], al[4];
+        const int off = (lane & 15) * ap + (lane >> 4) * 8;
+        ldsm4(a, smem_u32(as + off));
+        if (LOW) ldsm4(al, smem_u32(as_lo + off));
+        const int boff = ((lane & 7) + (lane >> 4) * 8) * bp + ((lane >> 3) & 1) * 8;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) h[r] = s * d.scale[w];
+        for (int i = 0; i < NBLK; i += 2) {
+            if (i >= blocks) break;
+            uint32_t b[4];
+            ldsm4(b, smem_u32(bs + i * 8 * bp + boff));
+            if (LOW) {
+                mma16<T>(d[i], al, b[0], b[1]);
+                mma16<T>(d[i + 1], al, b[2], b[3]);
+            }
+            mma16<T>(d[i], a, b[0], b[1]);
+            mma16<T>(d[i + 1], a, b[2], b[3]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 16; k += 8) {
+            uint32_t ah[4], al[4];
+            split_tf32(as[g * ap + k + t], ah[0], al[0]);
+            split_tf32(as[(g + 8) * ap + k + t], ah[1], al[1]);
+            split_tf32(as[g * ap + k + t + 4], ah[2], al[2]);
+            split_tf32(as[(g + 8) * ap + k + t + 4], ah[3], al[3]);
+#pragma unroll
+            for (int i = 0; i < NBLK; i++) {
+                if (i >= blocks) break;
+                const W* br = bs + (i * 8 + g) * bp + k + t;
+                uint32_t bh[2], bl[2];
+                split_tf32(to_f(br[0]), bh[0], bl[0]);
+                split_tf32(to_f(br[4]), bh[1], bl[1]);
+                mma8(d[i], al, bh[0], bh[1]);
+                if (is_f32<W>) mma8(d[i], ah, bl[0], bl[1]);
+                mma8(d[i], ah, bh[0], bh[1]);
+            }
+        }
     }
-    __syncthreads();
-    for (int n = threadIdx.x; n < d.N; n += kLoraThreads) {
-        float s = 0.0f;
-        for (int r = 0; r < rank; r++) s = fmaf(h[r], to_f(((const W*)d.b)[((int64_t)w * d.N + n) * d.rank + r]), s);
-        if (d.base) s += to_f(((const T*)d.base)[m * d.ldb + n]);
-        ((T*)d.out)[m * d.ldo + n] = from_f<T>(s);
+}
+
+// NW columns of B[w] from n0 on, [column][rank], to shared memory; zeros past
+// N and past the adapter's own rank r (what lies there may be anything).
+template <typename W, int NB>
+__device__ __forceinline__ void load_b(W* dst, int bp, const W* b, int n0, int N, int rank, int r, int Rp) {
+    constexpr int E = 16 / sizeof(W);
+    const int per = Rp / E;
+    for (int i = threadIdx.x; i < NB * per; i += kLoraThreads) {
+        const int row = i / per, c = (i - row * per) * E;
+        const bool ok = n0 + row < N && c < r;
+        const W* src = b + (int64_t)(ok ? n0 + row : 0) * rank + (ok ? c : 0);
+        if (ok && c + E > r) {  // the adapter's rank ends inside these 16 bytes
+            uint4 v = *reinterpret_cast<const uint4*>(src);
+            W e[E];
+            memcpy(e, &v, 16);
+#pragma unroll
+            for (int j = 0; j < E; j++)
+                if (c + j >= r) e[j] = from_f<W>(0.0f);
+            memcpy(&v, e, 16);
+            *reinterpret_cast<uint4*>(dst + row * bp + c) = v;
+        } else {
+            cp_async16_or_zero(dst + row * bp + c, src, ok);
+        }
     }
+}
+
+// One cluster per tile of up to TM rows of one request, both products in one
+// launch.  The CTAs of the cluster split K for h = x A^T (chunks of KB, two
+// cp.async stages), add their partial sums of h through each other's shared
+// memory in rank order, and split the columns for out = base + scale h B^T.
+// The traffic is x, base, out and the weights once: bound by HBM for prompts
+// and by the latency of one chain (tile, x and A, cluster barrier, store) for
+// single tokens, so the first columns of B are already on their way during
+// the first product.  TM 16 puts the four warps along K and the columns (a
+// step's tile has one row), TM 64 along the rows.  Both sums are fp32; h
+// enters the second product unrounded to 16 significant bits or more (two
+// 16-bit parts, or TF32 parts), because a 16-bit h would cost as much accuracy
+// as the output's own rounding.
+template <typename T, typename W, int TM, int RB>
+__global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constant__ voxq_lora d) {
+    using S = LoraShape<T, W, TM>;
+    constexpr int WM = S::WM, WK = S::WK, KB = S::KB, NB = S::NB, NW = S::NW;
+    extern __shared__ __align__(16) uint8_t lora_sh[];
+    const S z(d.rank);
+    uint32_t crank, csize;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(crank));
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
+    const int tile = blockIdx.x / csize;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wm = warp % WM, wk = warp / WM;
+    pdl_wait();
+    pdl_launch_dependents();
+
+    // Request s owns tiles cu[s] / TM + s on (as many as it can need, with
+    // gaps), so the tile's request is found without a scan: the last s whose
+    // first tile is not past this one.
+    int s = -1;
+    for (int i0 = 0; i0 < d.batch; i0 += kLoraThreads) {
+        const int i = i0 + threadIdx.x;
+        s += __syncthreads_count(i < d.batch && __ldg(d.cu + i) / TM + i <= tile);
+    }
+    s = max(s, 0);
+    const int first = __ldg(d.cu + s), m0 = first + (tile - (first / TM + s)) * TM;
+    const int rows = min(min(__ldg(d.cu + s + 1), d.rows) - m0, TM);
+    if (rows <= 0 || m0 < 0) return;  // the whole cluster
+    const int w = __ldg(d.adapter + s);
+    const bool on = w >= 0 && w < d.adapters;
+    const int r = !on ? 0 : d.ranks ? min(max(__ldg(d.ranks + w), 0), d.rank) : d.rank;
+    const W* wa = (const W*)d.a + (int64_t)w * d.rank * d.K;
+    const W* wb = (const W*)d.b + (int64_t)w * d.N * d.rank;
+    const int blocks = (r + 7) / 8, inner = (r + 15) / 16;
+
+    W* bs0 = reinterpret_cast<W*>(lora_sh + z.o_b0);
+    T* hs = reinterpret_cast<T*>(lora_sh + z.o_hs);  // h as two 16-bit parts, or fp32
+    T* hs_lo = hs + (is_f32<T> ? 0 : TM * z.hp);
+    if (r > 0) {
+        load_b<W, NB>(bs0, z.bp, wb, crank * NB, d.N, d.rank, r, z.Rp);
+        cp_async_commit();
+        const int chunks = (d.K + KB - 1) / KB, mine = chunks > (int)crank ? (chunks - crank + csize - 1) / csize : 0;
+        auto fetch = [&](int c) {
+            T* xs = reinterpret_cast<T*>(lora_sh + (c & 1) * z.stage);
+            W* as = reinterpret_cast<W*>(xs + TM * S::XP);
+            const int k0 = (crank + c * csize) * KB;
+            constexpr int EX = 16 / sizeof(T), EA = 16 / sizeof(W);
+            for (int i = threadIdx.x; i < TM * (KB / EX); i += kLoraThreads) {
+                const int row = i / (KB / EX), col = i % (KB / EX) * EX;
+                const bool ok = row < rows && k0 + col < d.K;
+                cp_async16_or_zero(xs + row * S::XP + col, (const T*)d.x + (ok ? (m0 + row) * d.ldx + k0 + col : 0), ok);
+            }
+            for (int i = threadIdx.x; i < z.Rp * (KB / EA); i += kLoraThreads) {
+                const int row = i / (KB / EA), col = i % (KB / EA) * EA;
+                const bool ok = row < r && k0 + col < d.K;
+                cp_async16_or_zero(as + row * S::AP + col, wa + (ok ? (int64_t)row * d.K + k0 + col : 0), ok);
+            }
+        };
+        float acc[RB][4];
+#pragma unroll
+        for (int i = 0; i < RB; i++) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+        if (mine > 0) fetch(0);
+        cp_async_commit();
+        for (int c = 0; c < mine; c++) {
+            if (c + 1 < mine) fetch(c + 1);
+            cp_async_commit();
+            cp_async_wait<1>();
+            __syncthreads();
+            const T* xs = reinterpret_cast<const T*>(lora_sh + (c & 1) * z.stage) + wm * 16 * S::XP;
+            const W* as = reinterpret_cast<const W*>(reinterpret_cast<const T*>(lora_sh + (c & 1) * z.stage) + TM * S::XP);
+            for (int k = wk * 16; k < KB; k += WK * 16)
+                mul_16<T, W, RB, false>(acc, xs + k, nullptr, S::XP, as + k, S::AP, blocks);
+            __syncthreads();
+        }
+        // this CTA's part of h: [K part of a warp][row][rank]
+        float* hp = reinterpret_cast<float*>(lora_sh + z.o_hpart);
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int i = 0; i < RB; i++) {
+            if (i >= blocks) break;
+            float* at = hp + (wk * TM + wm * 16 + g) * z.hp + i * 8 + 2 * t;
+            *reinterpret_cast<float2*>(at) = make_float2(acc[i][0], acc[i][1]);
+            *reinterpret_cast<float2*>(at + 8 * z.hp) = make_float2(acc[i][2], acc[i][3]);
+        }
+        if (WK > 1) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < rows * blocks * 8; i += kLoraThreads) {
+                const int at = i / (blocks * 8) * z.hp + i % (blocks * 8);
+                float v = hp[at];
+#pragma unroll
+                for (int j = 1; j < WK; j++) v += hp[j * TM * z.hp + at];
+                hp[at] = v;
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        // every CTA takes the whole of h: the parts in rank order, four values a step
+        const float scale = __ldg(d.scale + w);
+        const uint32_t local = smem_u32(hp);
+        for (int i = threadIdx.x; i < TM * (z.Rp / 4); i += kLoraThreads) {
+            const int row = i / (z.Rp / 4), col = i % (z.Rp / 4) * 4;
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (row < rows && col < r)
+                for (uint32_t c = 0; c < csize; c++) {
+                    uint32_t addr;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(local + (row * z.hp + col) * 4), "r"(c));
+                    float p[4];
+                    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                                 : "=f"(p[0]), "=f"(p[1]), "=f"(p[2]), "=f"(p[3]) : "r"(addr) : "memory");
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v[j] += p[j];
+                }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float h = col + j < r ? v[j] * scale : 0.0f;
+                hs[row * z.hp + col + j] = from_f<T>(h);
+                if constexpr (!is_f32<T>) hs_lo[row * z.hp + col + j] = from_f<T>(h - to_f(from_f<T>(h)));
+            }
+        }
+        // peers may still read this CTA's part: no CTA leaves before all have arrived here
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    }
+
+    // Columns n0 .. n0 + NB - 1 at a time; a warp owns 16 rows x NW columns of
+    // them and turns its fragments into rows through its own staging, so that
+    // base and out move in 16-byte accesses.
+    constexpr int E = 16 / sizeof(T), PER = 16 * NW / E / 32;
+    float* ost = reinterpret_cast<float*>(lora_sh + z.o_out) + warp * 16 * S::OP;
+    W* bs1 = reinterpret_cast<W*>(lora_sh + z.o_b1);
+    const int step = csize * NB;
+    int it = 0;
+    for (int n0 = crank * NB; n0 < d.N; n0 += step, it++) {
+        const int nw = n0 + (WK > 1 ? wk * NW : 0);
+        uint4 old[PER];
+        bool ok[PER];
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int i = lane + 32 * j, row = wm * 16 + i / (NW / E), col = nw + i % (NW / E) * E;
+            ok[j] = row < rows && col < d.N;
+            old[j] = make_uint4(0, 0, 0, 0);
+            if (ok[j] && d.base) old[j] = *reinterpret_cast<const uint4*>((const T*)d.base + (m0 + row) * d.ldb + col);
+        }
+        if (r > 0) {
+            cp_async_wait<0>();
+            __syncthreads();  // this step's B has landed (and h is written); the other buffer is free
+            if (n0 + step < d.N) load_b<W, NB>(it & 1 ? bs0 : bs1, z.bp, wb, n0 + step, d.N, d.rank, r, z.Rp);
+            cp_async_commit();
+            const W* bs = (it & 1 ? bs1 : bs0) + (WK > 1 ? wk * NW * z.bp : 0);
+            float o[NW / 8][4];
+#pragma unroll
+            for (int i = 0; i < NW / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+            for (int k = 0; k < inner; k++)
+                mul_16<T, W, NW / 8, !is_f32<T>>(o, hs + wm * 16 * z.hp + k * 16, hs_lo + wm * 16 * z.hp + k * 16, z.hp,
+                                                 bs + k * 16, z.bp, NW / 8);
+            const int g = lane >> 2, t = lane & 3;
+            __syncwarp();  // the last step's rows are read
+#pragma unroll
+            for (int i = 0; i < NW / 8; i++) {
+                *reinterpret_cast<float2*>(ost + g * S::OP + i * 8 + 2 * t) = make_float2(o[i][0], o[i][1]);
+                *reinterpret_cast<float2*>(ost + (g + 8) * S::OP + i * 8 + 2 * t) = make_float2(o[i][2], o[i][3]);
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            if (!ok[j]) continue;
+            const int i = lane + 32 * j, lr = i / (NW / E), lc = i % (NW / E) * E;
+            if (r > 0) {
+                T e[E];
+                memcpy(e, &old[j], 16);
+#pragma unroll
+                for (int v = 0; v < E; v += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(ost + lr * S::OP + lc + v);
+                    e[v] = from_f<T>(to_f(e[v]) + f.x);
+                    e[v + 1] = from_f<T>(to_f(e[v + 1]) + f.y);
+                    e[v + 2] = from_f<T>(to_f(e[v + 2]) + f.z);
+                    e[v + 3] = from_f<T>(to_f(e[v + 3]) + f.w);
+                }
+                memcpy(&old[j], e, 16);
+            }
+            *reinterpret_cast<uint4*>((T*)d.out + (m0 + wm * 16 + lr) * d.ldo + nw + lc) = old[j];
+        }
+    }
+    cp_async_wait<0>();
+    if (r > 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <typename T, typename W, int TM, int RB>
+static VoxCPMError lora_launch(const voxq_lora& d, cudaStream_t st) {
+    const LoraShape<T, W, TM> z(d.rank);
+    static std::once_flag once;
+    static cudaError_t attr = cudaSuccess;
+    auto kern = lora_kernel<T, W, TM, RB>;
+    std::call_once(once, [&] {
+        attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, LoraShape<T, W, TM>(RB * 8).bytes);
+    });
+    VOXQ_CUDA_TRY(attr);
+    // as many CTAs to a tile as it takes to fill the GPU twice, up to 8
+    const int tiles = d.rows / TM + d.batch;
+    int cl = 8;
+    while (cl > 1 && (int64_t)tiles * cl > 4 * device_sm_count()) cl /= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(tiles * cl);
+    cfg.blockDim = dim3(kLoraThreads);
+    cfg.dynamicSmemBytes = z.bytes;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cl;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    VOXQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, d));
+    return VOXCPM_SUCCESS;
+}
+
+// Tiles of 64 rows read the weights less often, tiles of 16 waste fewer rows
+// on requests of a few.
+template <typename T, typename W>
+static VoxCPMError lora_dispatch(const voxq_lora& d, cudaStream_t st) {
+    const bool tall = d.rows >= 24 * (int64_t)d.batch;
+    if (d.rank <= 32) return tall ? lora_launch<T, W, 64, 4>(d, st) : lora_launch<T, W, 16, 4>(d, st);
+    return tall ? lora_launch<T, W, 64, 16>(d, st) : lora_launch<T, W, 16, 16>(d, st);
 }
 
 }  // namespace voxq
@@ -65,9 +408,12 @@ extern "C" VoxCPMError voxq_lora_forward(const voxq_lora* d, void* stream) {
     voxq_lora p = *d;
     if (!weights) p.adapters = 0;
     cudaStream_t st = (cudaStream_t)stream;
-    with_elem(p.dtype, [&](auto x) {
-        with_elem(p.w_dtype, [&](auto w) { lora_kernel<decltype(x), decltype(w)><<<p.rows, kLoraThreads, 0, st>>>(p); });
+    return with_elem(p.dtype, [&](auto x) {
+        return with_elem(p.w_dtype, [&](auto w) {
+            using T = decltype(x);
+            using W = decltype(w);
+            if constexpr (is_f32<T> || std::is_same<T, W>::value) return lora_dispatch<T, W>(p, st);
+            else return VOXCPM_ERR_UNSUPPORTED;
+        });
     });
-    VOXQ_CUDA_TRY(cudaGetLastError());
-    return VOXCPM_SUCCESS;
 }

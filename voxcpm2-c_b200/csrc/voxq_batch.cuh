@@ -5,6 +5,8 @@
 
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "voxq_common.cuh"
 #include "voxq_internal.h"
 
@@ -51,12 +53,64 @@ inline cudaError_t launch_pdl(void (*kern)(P...), dim3 grid, dim3 block, size_t 
     return cudaLaunchKernelEx(&cfg, kern, P(args)...);
 }
 
+template <typename T>
+constexpr bool is_f32 = std::is_same<T, float>::value;
+
+// 16 bytes to shared memory, zeros when !ok (the source is then not read).
+__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// x as a sum of two TF32 values: what is left out is below 2^-22 of it.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    const float r = x - __uint_as_float(hi);
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(r));
+}
+
 // Calls f with a value of the element type that `dtype` names.
 template <typename F>
 auto with_elem(int dtype, F f) {
     if (dtype == VOXQ_F16) return f(__half{});
     if (dtype == VOXQ_BF16) return f(bf16{});
     return f(float{});
+}
+
+// The request (or sequence) whose rows fill tile `tile` of a ragged batch, when
+// the items of request s own tiles cu[s] * mul / TM + s on: as many as they can
+// need, with gaps, so no scan is needed -- it is the last s whose first tile is
+// not past this one.  All threads of the block take part; batch > 0.
+template <int TM>
+__device__ __forceinline__ int tile_owner(const int32_t* __restrict__ cu, int batch, int mul, int tile) {
+    int s = -1;
+    for (int i0 = 0; i0 < batch; i0 += blockDim.x) {
+        const int i = i0 + threadIdx.x;
+        s += __syncthreads_count(i < batch && __ldg(cu + i) * mul / TM + i <= tile);
+    }
+    return max(s, 0);
 }
 
 }  // namespace voxq

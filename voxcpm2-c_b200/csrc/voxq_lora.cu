@@ -11,9 +11,6 @@ constexpr int kLoraThreads = 128;
 constexpr int kLoraWarps = kLoraThreads / 32;
 constexpr int kLoraMaxRank = 128;
 
-template <typename T>
-constexpr bool is_f32 = std::is_same<T, float>::value;
-
 // Shape of the kernel for x of type T, weights of type W and TM rows a tile.
 template <typename T, typename W, int TM>
 struct LoraShape {
@@ -44,41 +41,6 @@ struct LoraShape {
         bytes = o_b0 + bbytes;
     }
 };
-
-// 16 bytes to shared memory, zeros when !ok (the source is then not read).
-__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool ok) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
-
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-
-template <typename T>
-__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (std::is_same<T, __half>::value)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// x as a sum of two TF32 values: what is left out is below 2^-22 of it.
-__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    const float r = x - __uint_as_float(hi);
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(r));
-}
 
 // d[i] += a b[i]^T over 16 of the inner dimension, the 16 x 16 a at `as` and NBLK 8-row blocks of b at `bs`, both in
 // shared memory with the inner dimension contiguous.  16-bit: one MMA per block (and one more for a's low part at
@@ -178,15 +140,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
     pdl_wait();
     pdl_launch_dependents();
 
-    // Request s owns tiles cu[s] / TM + s on (as many as it can need, with
-    // gaps), so the tile's request is found without a scan: the last s whose
-    // first tile is not past this one.
-    int s = -1;
-    for (int i0 = 0; i0 < d.batch; i0 += kLoraThreads) {
-        const int i = i0 + threadIdx.x;
-        s += __syncthreads_count(i < d.batch && __ldg(d.cu + i) / TM + i <= tile);
-    }
-    s = max(s, 0);
+    const int s = tile_owner<TM>(d.cu, d.batch, 1, tile);
     const int first = __ldg(d.cu + s), m0 = first + (tile - (first / TM + s)) * TM;
     const int rows = min(min(__ldg(d.cu + s + 1), d.rows) - m0, TM);
     if (rows <= 0 || m0 < 0) return;  // the whole cluster

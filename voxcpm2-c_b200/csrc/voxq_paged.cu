@@ -4,61 +4,18 @@
 #include <algorithm>
 #include <mutex>
 
-#include "voxq_batch.cuh"
 #include "voxq_internal.h"
+#include "voxq_paged.cuh"
 
 namespace voxq {
 
 constexpr int kPagedThreads = 128;
 constexpr int kPagedMaxHeadDim = 256;
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kSplitCtas = 4;   // CTAs per SM that splitting the keys aims at
+constexpr int kTcSplitCtas = 1;  // the same for the tcgen05 kernel, one CTA of which fills an SM
+constexpr int kTcMinRows = 64;   // rows a sequence from which that kernel's 128-row tiles pay
 constexpr int kMinSplit = 256;  // keys that are worth a CTA of their own
 constexpr int kMaxSplits = 128;
-
-// The call's sizes as the kernels take them.
-struct PagedArgs {
-    voxq_paged_attn d;
-    int group;        // query heads per kv head
-    int page_shift;   // log2(page_size), or -1
-    int split_len;    // keys per split (a multiple of the key tile)
-    int splits;       // most splits a row can have; 1: none
-    float scale2;     // scale * log2(e): the softmax runs in base 2
-    float2* ml;       // [total_q][heads][splits] running maximum and sum
-    float* acc;       // [total_q][heads][splits][head_dim] unnormalised sums
-};
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Offset of cache position j of a sequence (its block-table row `table`) at
-// kv head kh, in elements.
-__device__ __forceinline__ int64_t cache_row(const PagedArgs& p, const int32_t* table, int j, int kh) {
-    const int e = p.page_shift >= 0 ? j >> p.page_shift : (int)((uint32_t)j / (uint32_t)p.d.page_size);
-    const int page = __ldg(table + e);
-    return (int64_t)((uint32_t)page < (uint32_t)p.d.pages ? page : 0) * p.d.page_stride +
-           (int64_t)(j - e * p.d.page_size) * p.d.row_stride + (int64_t)kh * p.d.head_stride;
-}
-
-// Positions that row i of a sequence's n sees.
-__device__ __forceinline__ int visible(const PagedArgs& p, int len, int n, int i) {
-    return p.d.causal ? max(min(len, len - n + i + 1), 0) : len;
-}
-
-template <typename T>
-__device__ __forceinline__ void store_pair(const PagedArgs& p, int64_t at, float x, float y) {
-    if (is_f32<T> || p.d.out_dtype == VOXQ_F32) {
-        *reinterpret_cast<float2*>((float*)p.d.out + at) = make_float2(x, y);
-    } else {
-        T e[2] = {from_f<T>(x), from_f<T>(y)};
-        uint32_t v;
-        memcpy(&v, e, 4);
-        *reinterpret_cast<uint32_t*>((T*)p.d.out + at) = v;
-    }
-}
 
 // Shape of the kernel for element type T, head dims up to HD and WM warps
 // along the rows (the other 4 / WM along the keys of a tile).
@@ -423,7 +380,8 @@ __global__ void __launch_bounds__(kPagedThreads) paged_combine_kernel(const __gr
 // What a call runs: rows per tile, and the keys per split.  A pure function of
 // the descriptor's integers, so that the workspace is known beforehand.
 struct PagedPlan {
-    int wm;         // warps along the rows
+    bool tc;        // tcgen05 kernel
+    int wm;         // warps along the rows of the other
     int split_len, splits;
     size_t bytes;   // workspace
 };
@@ -433,14 +391,15 @@ static PagedPlan paged_plan(const voxq_paged_attn& d) {
     const int G = d.heads / d.kv_heads;
     // 16-row tiles while a sequence's rows fit in one
     r.wm = (int64_t)d.max_q * G <= 16 ? 1 : 4;
-    const int tr = 16 * r.wm;
+    r.tc = (int64_t)d.max_q * G > kTcMinRows && paged_tc_takes(d);
+    const int tr = r.tc ? kTcRows : 16 * r.wm, ctas = r.tc ? kTcSplitCtas : kSplitCtas;
     // CTAs without splitting, and the splits that bring them to kSplitCtas per SM
     const int64_t per_seq = std::max<int64_t>(1, std::min<int64_t>(d.batch, d.total_q));
     const int64_t tiles = std::max<int64_t>(per_seq, (int64_t)d.total_q * G / tr) * d.kv_heads;
-    const int64_t want = (kSplitCtas * device_sm_count() + tiles - 1) / tiles;
+    const int64_t want = (ctas * device_sm_count() + tiles - 1) / tiles;
     const int64_t most = std::max<int64_t>(1, (d.max_kv + kMinSplit - 1) / kMinSplit);
     const int64_t z = std::min(std::min(want, most), (int64_t)kMaxSplits);
-    r.split_len = (int)(((d.max_kv + z - 1) / z + 63) / 64 * 64);
+    r.split_len = (int)(((d.max_kv + z - 1) / z + 127) / 128 * 128);  // whole tiles of either kernel
     r.splits = r.split_len ? (d.max_kv + r.split_len - 1) / r.split_len : 1;
     if (r.splits <= 1) {
         r.splits = 1;
@@ -466,10 +425,11 @@ static VoxCPMError paged_mma_launch(const PagedArgs& a, cudaStream_t st) {
 template <typename T>
 static VoxCPMError paged_run(const PagedArgs& a, const PagedPlan& plan, cudaStream_t st) {
     const int hd = a.d.head_dim;
-    VoxCPMError e;
-    if (plan.wm == 1)
+    // (a cache layout that a tensor map cannot describe goes to the other kernel)
+    VoxCPMError e = plan.tc ? paged_tc_launch(a, st) : VOXCPM_ERR_UNSUPPORTED;
+    if (e == VOXCPM_ERR_UNSUPPORTED && plan.wm == 1)
         e = hd <= 64 ? paged_mma_launch<T, 64, 1>(a, st) : hd <= 128 ? paged_mma_launch<T, 128, 1>(a, st) : paged_mma_launch<T, 256, 1>(a, st);
-    else
+    else if (e == VOXCPM_ERR_UNSUPPORTED)
         e = hd <= 64 ? paged_mma_launch<T, 64, 4>(a, st) : hd <= 128 ? paged_mma_launch<T, 128, 4>(a, st) : paged_mma_launch<T, 256, 4>(a, st);
     if (e != VOXCPM_SUCCESS || a.splits == 1) return e;
     const int per = a.d.heads * hd / 2, y = std::min(8, (per + kPagedThreads - 1) / kPagedThreads);

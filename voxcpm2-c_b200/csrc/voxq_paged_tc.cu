@@ -53,6 +53,12 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
 #define VOXQ_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
 #define VOXQ_S8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
 // 32 columns of this thread's tensor-memory lane; the caller waits.
@@ -126,7 +132,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     __shared__ uint32_t tmem_slot;
     uint64_t *full = bar, *empty = bar + ST, *s_full = bar + 2 * ST, *p_full = s_full + 2, *o_done = p_full + 2, *q_full = o_done + 2;
     const voxq_paged_attn& d = p.d;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.group, kh = blockIdx.y;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, G = p.group, kh = blockIdx.y;
     const uint32_t qsm = (smem_u32(tc_raw) + 1023) & ~1023u, ring = qsm + 2 * TILE;
     pdl_wait();
     pdl_launch_dependents();
@@ -164,7 +170,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     tc_before();
     __syncthreads();
     tc_after();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
 
     if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcRegsOther));
@@ -198,12 +204,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         // ---------------- MMA issue ----------------
         constexpr uint32_t id_s = tc_idesc<T>(kTcTile, false), id_o = tc_idesc<T>(HD, true);
         bool ok = tiles == 0 || warp_wait(q_full, 0, VOXQ_DEVERR_WAIT_FULL, maps.err);
+        // One lane issues; the operands are the same in every lane, so that they stay in uniform registers.
+        const bool one = elect_one();
         auto scores = [&](int t, int slot) {
-            if (lane == 0) {
+            const uint64_t qd = desc_k(qsm + t * TILE), kd = desc_k(ring + slot * TILE);
+            if (one) {
 #pragma unroll
                 for (int k = 0; k < HD / 16; k++) {
-                    const uint32_t off = (k / 4) * kTcHalf + (k % 4) * 32;
-                    mma_ss(tmem + t * kTcTile, desc_k(qsm + t * TILE + off), desc_k(ring + slot * TILE + off), id_s, k > 0);
+                    const uint32_t off = ((k / 4) * kTcHalf + (k % 4) * 32) >> 4;
+                    mma_ss(tmem + t * kTcTile, qd + off, kd + off, id_s, k > 0);
                 }
                 tc_commit(s_full + t);
             }
@@ -214,7 +223,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             if (ok) {
                 scores(0, 0);
                 if (two) scores(1, 0);
-                if (lane == 0) tc_commit(empty + 0);
+                if (one) tc_commit(empty + 0);
             }
         }
         for (int i = 0; i < tiles && ok; i++) {
@@ -237,17 +246,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 ok = warp_wait(p_full + t, i & 1, VOXQ_DEVERR_WAIT_MMA, maps.err);
                 if (!ok) break;
                 tc_after();
-                if (lane == 0)
-                    for (int k = 0; k < steps; k++)
-                        mma_ts(tmem + 256 + t * HD, tmem + t * kTcTile + k * 8, desc_mn(ring + sv * TILE + k * 2048), id_o, i > 0 || k > 0);
+                const uint64_t vd = desc_mn(ring + sv * TILE);
+                if (one) {
+#pragma unroll
+                    for (int k = 0; k < kTcTile / 16; k++)
+                        if (k < steps) mma_ts(tmem + 256 + t * HD, tmem + t * kTcTile + k * 8, vd + (k * 2048 >> 4), id_o, i > 0 || k > 0);
+                }
                 if (i + 1 < tiles) {
                     if (t == 0) ok = warp_wait(full + sk, (ck / ST) & 1, VOXQ_DEVERR_WAIT_FULL, maps.err);
                     if (ok) scores(t, sk);
-                } else if (lane == 0) {
+                } else if (one) {
                     tc_commit(o_done + t);
                 }
             }
-            if (lane == 0 && i + 1 < tiles) {  // (after the last tile nothing waits for them)
+            if (one && i + 1 < tiles) {  // (after the last tile nothing waits for them)
                 tc_commit(empty + sv);
                 tc_commit(empty + sk);
             }

@@ -168,6 +168,19 @@ def test_paged_attention_offsets_past_32_bits():
         del k, v
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+def test_paged_attention_many_units(causal, dim, dtype):
+    """More row tiles than the GPU has SMs, of very different lengths, and more sequences than one search pass takes:
+    every block goes through several units."""
+    rng = random.Random(dim)
+    n = [700, 0, 1, 1100] + [rng.randint(1, 90) for _ in range(30)]
+    attend(n, [a + rng.randint(0, 200) for a in n], 48, 3, dim, 16, dtype, causal, seed=dim)
+    n = [rng.randint(9, 30) for _ in range(150)]
+    attend(n, [a + rng.randint(0, 300) for a in n], 16, 2, dim, 16, dtype, causal, seed=dim)
+
+
 @pytest.mark.parametrize("n,lens", [([1] * 5, [3000, 20, 400, 1, 800]), ([190, 40], [300, 2500])])
 def test_paged_attention_same_bits_and_other_streams(n, lens):
     """The same bits on every run, on a side stream and inside a CUDA graph."""

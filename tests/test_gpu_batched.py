@@ -205,6 +205,29 @@ def test_paged_attention_same_bits_and_other_streams(n, lens):
     assert torch.equal(first, out)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("batch,top", [(64, 1500), (3, 20000)])
+def test_paged_attention_long_steps(batch, top, dim, dtype):
+    """Next-token steps whose splits hold many more tiles than a block has stages, several times over."""
+    rng = random.Random(batch)
+    lens = [rng.randint(top // 3, top) for _ in range(batch)]
+    pool = Pool(lens, 16, 2, dim, dtype)
+    q = torch.randn(batch, 16, dim, device="cuda").to(dtype)
+    cu, kv = ints(range(batch + 1)), ints(lens)
+    first = None
+    for _ in range(5):
+        o = voxq.paged_attention(q, pool.k, pool.v, pool.table, cu, kv, 1, max(lens))
+        first = o if first is None else first
+        assert torch.equal(first, o)
+    some = sorted(rng.sample(range(batch), min(batch, 5)))
+    at = torch.tensor(some, device="cuda")
+    ref, bound = R.attention(q[at], torch.nan_to_num(pool.k), torch.nan_to_num(pool.v), pool.table[at], ints(range(len(some) + 1)),
+                             kv[at], True, dim ** -0.5)
+    R.assert_within(first[at], ref, bound)
+    assert int(voxq.lib().voxq_device_error(1)) == 0
+
+
 def test_paged_attention_batch_equals_alone():
     """A sequence's step does not depend on who shares the batch, up to the split of its keys over CTAs."""
     lens = [900, 33, 2100]

@@ -2,6 +2,8 @@
 // the walk through the block table, the causal limit and the output types.
 #pragma once
 
+#include <cuda.h>
+
 #include "voxq_batch.cuh"
 
 namespace voxq {
@@ -18,6 +20,7 @@ struct PagedArgs {
     float scale2;     // scale * log2(e): the softmax runs in base 2
     float2* ml;       // [total_q][heads][splits] running maximum and sum
     float* acc;       // [total_q][heads][splits][head_dim] unnormalised sums
+    int* err;         // device error word of the bounded waits
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -52,8 +55,179 @@ __device__ __forceinline__ void store_pair(const PagedArgs& p, int64_t at, float
     }
 }
 
-// Attention on the tcgen05 tensor cores (voxq_paged_tc.cu): 16-bit types, head_dim 64 or 128, page_size a multiple
-// of 8, scale > 0.  Launches the main kernel only.
+__device__ __forceinline__ float lds_f32(uint32_t a) { return __uint_as_float(lds32(a)); }
+
+// Rows of P elements at a shared address.
+template <typename T, int P>
+struct PaddedRows {
+    uint32_t base;
+    __device__ __forceinline__ uint32_t operator()(int row, int dim) const { return base + (row * P + dim) * (int)sizeof(T); }
+};
+
+// One step of a warp: its 16 rows against 8 KN keys.  16-bit types: m16n8k16 with fp32 accumulation; the weights p
+// enter the second product as two 16-bit parts, since one would cost as much accuracy as the output's own rounding.
+// fp32: three TF32 products per operand pair (high and low parts), the second product's sums started afresh each step
+// and added in fp32, because MMA accumulation truncates.  qs: the rows' queries in shared memory (16-bit types with
+// HD <= 128 take them from the registers qf instead), pitch HD + 16 bytes; ks(row, dim), vs(row, dim): shared addresses
+// of the keys and values; base: the position
+// of this lane's first score column (2 t into the keys); vis: what rows g and g + 8 see; m, l, o: running maxima, this
+// lane's share of the sums, and outputs.
+template <typename T, int HD, int KN, int QN, typename A>
+__device__ __forceinline__ void attend_keys(const PagedArgs& p, const T* qs, const uint32_t (&qf)[QN][4], const A& ks, const A& vs, int base,
+                                            const int (&vis)[2], float (&m)[2], float (&l)[2], float (&o)[HD / 8][4]) {
+    constexpr int NB = HD / 8, P = HD + 16 / (int)sizeof(T);
+    constexpr bool QREG = QN > 1;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    float sc[KN][4];
+#pragma unroll
+    for (int j = 0; j < KN; j++) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
+    if constexpr (!is_f32<T>) {
+#pragma unroll
+        for (int k = 0; k < HD / 16; k++) {
+            uint32_t a[4];
+            if constexpr (QREG) {
+                a[0] = qf[k][0], a[1] = qf[k][1], a[2] = qf[k][2], a[3] = qf[k][3];
+            } else {
+                ldsm4(a, smem_u32(qs + (lane & 15) * P + k * 16 + (lane >> 4) * 8));
+            }
+#pragma unroll
+            for (int j = 0; j < KN; j += 2) {
+                uint32_t b[4];
+                ldsm4(b, ks(j * 8 + (lane & 7) + (lane >> 4) * 8, k * 16 + ((lane >> 3) & 1) * 8));
+                mma16<T>(sc[j], a, b[0], b[1]);
+                mma16<T>(sc[j + 1], a, b[2], b[3]);
+            }
+        }
+    } else {
+#pragma unroll 4
+        for (int k = 0; k < HD; k += 8) {
+            uint32_t ah[4], al[4];
+            split_tf32(qs[g * P + k + t], ah[0], al[0]);
+            split_tf32(qs[(g + 8) * P + k + t], ah[1], al[1]);
+            split_tf32(qs[g * P + k + t + 4], ah[2], al[2]);
+            split_tf32(qs[(g + 8) * P + k + t + 4], ah[3], al[3]);
+#pragma unroll
+            for (int j = 0; j < KN; j++) {
+                uint32_t bh[2], bl[2];
+                split_tf32(lds_f32(ks(j * 8 + g, k + t)), bh[0], bl[0]);
+                split_tf32(lds_f32(ks(j * 8 + g, k + t + 4)), bh[1], bl[1]);
+                mma8(sc[j], al, bh[0], bh[1]);
+                mma8(sc[j], ah, bl[0], bl[1]);
+                mma8(sc[j], ah, bh[0], bh[1]);
+            }
+        }
+    }
+
+    // masks, the rows' maxima over the quad, weights
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int j = 0; j < KN; j++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            sc[j][c] = base + j * 8 + (c & 1) < vis[c >> 1] ? sc[j][c] * p.scale2 : -INFINITY;
+            mx[c >> 1] = fmaxf(mx[c >> 1], sc[j][c]);
+        }
+    float f[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+        mx[e] = fmaxf(fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2)), m[e]);
+        f[e] = m[e] == -INFINITY ? 0.0f : ex2(m[e] - mx[e]);
+        m[e] = mx[e];
+        mx[e] = mx[e] == -INFINITY ? 0.0f : mx[e];  // no key so far: every weight is ex2(-inf) = 0
+        l[e] *= f[e];
+    }
+#pragma unroll
+    for (int j = 0; j < KN; j++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            sc[j][c] = ex2(sc[j][c] - mx[c >> 1]);
+            l[c >> 1] += sc[j][c];
+        }
+
+    if constexpr (!is_f32<T>) {
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            o[j][0] *= f[0], o[j][1] *= f[0];
+            o[j][2] *= f[1], o[j][3] *= f[1];
+        }
+#pragma unroll
+        for (int k = 0; k < KN / 2; k++) {
+            uint32_t ph[4], pl[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float x = sc[2 * k + e / 2][e % 2 * 2], y = sc[2 * k + e / 2][e % 2 * 2 + 1];
+                const T hi[2] = {from_f<T>(x), from_f<T>(y)};
+                const T lo[2] = {from_f<T>(x - to_f(hi[0])), from_f<T>(y - to_f(hi[1]))};
+                memcpy(&ph[e], hi, 4);
+                memcpy(&pl[e], lo, 4);
+            }
+#pragma unroll
+            for (int j = 0; j < NB; j += 2) {
+                uint32_t b[4];
+                const uint32_t at = vs(k * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, j * 8 + (lane >> 4) * 8);
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]) : "r"(at) : "memory");
+                mma16<T>(o[j], pl, b[0], b[1]);
+                mma16<T>(o[j + 1], pl, b[2], b[3]);
+                mma16<T>(o[j], ph, b[0], b[1]);
+                mma16<T>(o[j + 1], ph, b[2], b[3]);
+            }
+        }
+    } else {
+        constexpr int NG = NB < 8 ? NB : 8;  // head-dim blocks whose sums are open at once
+#pragma unroll
+        for (int n0 = 0; n0 < NB; n0 += NG) {
+            float a[NG][4];
+#pragma unroll
+            for (int i = 0; i < NG; i++) a[i][0] = a[i][1] = a[i][2] = a[i][3] = 0.0f;
+            // A column t is key 2t and column t + 4 key 2t + 1 of the 8: the scores' own layout
+#pragma unroll
+            for (int j = 0; j < KN; j++) {
+                uint32_t ah[4], al[4];
+                split_tf32(sc[j][0], ah[0], al[0]);
+                split_tf32(sc[j][2], ah[1], al[1]);
+                split_tf32(sc[j][1], ah[2], al[2]);
+                split_tf32(sc[j][3], ah[3], al[3]);
+#pragma unroll
+                for (int i = 0; i < NG; i++) {
+                    uint32_t bh[2], bl[2];
+                    split_tf32(lds_f32(vs(j * 8 + 2 * t, g + (n0 + i) * 8)), bh[0], bl[0]);
+                    split_tf32(lds_f32(vs(j * 8 + 2 * t + 1, g + (n0 + i) * 8)), bh[1], bl[1]);
+                    mma8(a[i], al, bh[0], bh[1]);
+                    mma8(a[i], ah, bl[0], bl[1]);
+                    mma8(a[i], ah, bh[0], bh[1]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NG; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) o[n0 + i][c] = fmaf(o[n0 + i][c], f[c >> 1], a[i][c]);
+        }
+    }
+}
+
+// Tensor maps of a call's caches: boxes of 128 bytes of one head x box_rows rows of a page, 128-byte-swizzled.
+struct PagedMaps {
+    CUtensorMap k, v;
+    int box_rows;    // a power of two that divides page_size, at least 8, at most max_rows
+    int head_first;  // the map's order: dims, heads, rows, pages (else dims, rows, heads, pages), by their strides
+};
+// page_size a multiple of 8 and positive strides.
+bool paged_maps_take(const voxq_paged_attn& d);
+VoxCPMError paged_maps(const voxq_paged_attn& d, int max_rows, PagedMaps* m);
+// One box: dims x.., rows of a page from `row` on.
+__device__ __forceinline__ void tma_page(uint32_t dst, const PagedMaps& m, const CUtensorMap* map, int x, int row, int head, int page, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(m.head_first ? head : row), "r"(m.head_first ? row : head), "r"(page), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// At most 16 rows a sequence (voxq_paged_step.cu); head_dim as any, caches that paged_maps_take.
+VoxCPMError paged_step_launch(const PagedArgs& a, cudaStream_t st);
+// Attention on the tcgen05 tensor cores (voxq_paged_tc.cu): 16-bit types, head_dim 64 or 128, scale > 0, caches that
+// paged_maps_take.  Both launch the main kernel only and return VOXCPM_ERR_UNSUPPORTED for a layout that a tensor map
+// cannot describe.
 constexpr int kTcRows = 256;  // rows of a CTA
 bool paged_tc_takes(const voxq_paged_attn& d);
 VoxCPMError paged_tc_launch(const PagedArgs& a, cudaStream_t st);

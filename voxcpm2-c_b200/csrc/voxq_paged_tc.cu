@@ -121,12 +121,6 @@ __device__ __forceinline__ uint32_t pack2v(float x, float y) {  // x in the low 
     return r;
 }
 
-__device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int page, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(page), "r"(smem_u32(bar))
-                 : "memory");
-}
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float x, float y) {
     if constexpr (std::is_same<T, bf16>::value) {
@@ -142,13 +136,6 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int site, int* err) {
     return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, site, err));
 }
-
-struct TcMaps {
-    CUtensorMap k, v;
-    int box_rows;    // rows of a page that one copy takes: gcd(page_size, 128)
-    int head_first;  // the map's order: dims, heads, rows, pages (else dims, rows, heads, pages), by their strides
-    int* err;
-};
 
 // One unit of work: up to 256 rows of a sequence and kv head against one split of its keys.
 struct TcItem {
@@ -199,7 +186,7 @@ __device__ __forceinline__ bool next_block(const uint4* answer, int& x, int& y, 
 // the first scores of a unit run ahead of the previous one's output, and tensor memory, barriers and shared memory are
 // set up once.  Every wait is bounded and records the device error word.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ TcMaps maps) {
+__global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ PagedMaps maps) {
     constexpr int TILE = kTcTileBytes<HD>, ST = kTcStages;
     extern __shared__ uint8_t tc_raw[];
     __shared__ uint64_t bar[2 * ST + 2 * kTcItems + 12];
@@ -247,7 +234,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
 
     // The k-th unit; rows 0: no more.  done(k) frees its slot.
     auto unit_ready = [&](int k) {
-        return __all_sync(0xffffffffu, mbar_wait_bounded(item_full + k % kTcItems, (k / kTcItems) & 1, VOXQ_DEVERR_WAIT_FULL, maps.err, kTcLong));
+        return __all_sync(0xffffffffu, mbar_wait_bounded(item_full + k % kTcItems, (k / kTcItems) & 1, VOXQ_DEVERR_WAIT_FULL, p.err, kTcLong));
     };
     auto done = [&](int k) {
         __syncwarp();
@@ -277,7 +264,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 const int loads = 2 * it.tiles();
                 for (int i = 0; i < loads; i++, c++) {
                     const int slot = c % ST, t0 = it.k_beg + i / 2 * kTcTile;
-                    if (c >= ST) ok = warp_wait(empty + slot, (c / ST - 1) & 1, VOXQ_DEVERR_WAIT_EMPTY, maps.err);
+                    if (c >= ST) ok = warp_wait(empty + slot, (c / ST - 1) & 1, VOXQ_DEVERR_WAIT_EMPTY, p.err);
                     if (!ok) break;
                     // boxes that start before k_stop; the rest of the tile is masked
                     const int live = (min(it.k_stop - t0, kTcTile) + R - 1) / R * (HD / 64);
@@ -290,8 +277,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                         int page = __ldg(table + e);
                         if ((uint32_t)page >= (uint32_t)d.pages) page = 0;
                         const int off = key - e * d.page_size;
-                        tma_page(ring + slot * TILE + half * kTcHalf + row * 128, i & 1 ? &maps.v : &maps.k, half * 64,
-                                 maps.head_first ? it.kh : off, maps.head_first ? off : it.kh, page, full + slot);
+                        tma_page(ring + slot * TILE + half * kTcHalf + row * 128, maps, i & 1 ? &maps.v : &maps.k, half * 64, off, it.kh, page, full + slot);
                     }
                 }
                 const int odd = (it.k_stop - it.k_beg) % 16;
@@ -299,7 +285,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                     // The last 16 keys that enter the second product: what lies past the end may be anything, and
                     // 0 * NaN is NaN, so those rows become zeros.
                     const int slot = (c - 1) % ST, valid = (it.k_stop - it.k_beg) % kTcTile;
-                    ok = warp_wait(full + slot, ((c - 1) / ST) & 1, VOXQ_DEVERR_WAIT_FULL, maps.err);
+                    ok = warp_wait(full + slot, ((c - 1) / ST) & 1, VOXQ_DEVERR_WAIT_FULL, p.err);
                     for (int j = lane; ok && j < (16 - odd) * (HD / 8); j += 32) {
                         const int row = valid + j / (HD / 8), ch = j % (HD / 8);
                         sts128(ring + slot * TILE + (ch / 8) * kTcHalf + row * 128 + (ch % 8) * 16, make_uint4(0, 0, 0, 0));
@@ -311,7 +297,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 }
             }
             if (!ok)  // nothing of this block may still be writing its shared memory when it ends
-                for (uint32_t i = c > ST ? c - ST : 0; i < c; i++) mbar_wait_bounded(full + i % ST, (i / ST) & 1, VOXQ_DEVERR_NONE, maps.err);
+                for (uint32_t i = c > ST ? c - ST : 0; i < c; i++) mbar_wait_bounded(full + i % ST, (i / ST) & 1, VOXQ_DEVERR_NONE, p.err);
         } else if (warp == 9) {
             // ---------------- MMA issue ----------------
             // One thread, operands in uniform registers, few instructions between a barrier and the MMAs that wait for
@@ -323,7 +309,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             TcItem it;
             bool ok = true;
             uint32_t slot = 0, phase = 0, steps_done[2] = {0, 0}, units[2] = {0, 0}, tails = 0;
-            auto ready = [&] { return mbar_wait_bounded(full + slot, phase, VOXQ_DEVERR_WAIT_FULL, maps.err); };
+            auto ready = [&] { return mbar_wait_bounded(full + slot, phase, VOXQ_DEVERR_WAIT_FULL, p.err); };
             auto advance = [&] {
                 slot = slot + 1 == ST ? 0 : slot + 1;
                 phase ^= slot == 0;
@@ -352,7 +338,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
                     for (int t = 0; t < 2; t++) {
                         if (t && !two) break;
-                        ok = ok && mbar_wait_bounded(q_full + t, units[t]++ & 1, VOXQ_DEVERR_WAIT_FULL, maps.err, kTcLong);
+                        ok = ok && mbar_wait_bounded(q_full + t, units[t]++ & 1, VOXQ_DEVERR_WAIT_FULL, p.err, kTcLong);
                         tc_after();
                         if (ok) scores(t, sk);
                     }
@@ -368,7 +354,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                             sk = slot;
                             advance();
                         } else if (odd) {
-                            ok = ok && mbar_wait_bounded(tail + (tails & 1), (tails >> 1) & 1, VOXQ_DEVERR_WAIT_FULL, maps.err);
+                            ok = ok && mbar_wait_bounded(tail + (tails & 1), (tails >> 1) & 1, VOXQ_DEVERR_WAIT_FULL, p.err);
                             tails++;
                         }
                     };
@@ -381,7 +367,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
                         for (int t = 0; t < 2; t++) {
                             if (t && !two) break;
-                            ok = ok && mbar_wait_bounded(p_full + t, steps_done[t]++ & 1, VOXQ_DEVERR_WAIT_MMA, maps.err);
+                            ok = ok && mbar_wait_bounded(p_full + t, steps_done[t]++ & 1, VOXQ_DEVERR_WAIT_MMA, p.err);
                             tc_after();
                             if (!ok) break;
 #pragma unroll
@@ -407,7 +393,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             int x = blockIdx.x, y, z = blockIdx.z, k = 0;
             bool ok = true;
             auto put = [&](const TcItem& it) {
-                if (k >= kTcItems) ok = __all_sync(0xffffffffu, mbar_wait_bounded(item_empty + k % kTcItems, (k / kTcItems - 1) & 1, VOXQ_DEVERR_WAIT_EMPTY, maps.err, kTcLong));
+                if (k >= kTcItems) ok = __all_sync(0xffffffffu, mbar_wait_bounded(item_empty + k % kTcItems, (k / kTcItems - 1) & 1, VOXQ_DEVERR_WAIT_EMPTY, p.err, kTcLong));
                 if (lane == 0 && ok) {
                     items[k % kTcItems] = it;
                     mbar_arrive(item_full + k % kTcItems);
@@ -498,7 +484,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                         put(it);
                         // No unit is taken before the loader has come to this one: a block that reserved more would sit on
                         // them while others run out of work.
-                        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(begun, (k - 1) & 1, VOXQ_DEVERR_WAIT_EMPTY, maps.err, kTcLong));
+                        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(begun, (k - 1) & 1, VOXQ_DEVERR_WAIT_EMPTY, p.err, kTcLong));
                         if (!ok) break;
                     }
                 }
@@ -506,7 +492,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                     mbar_arrive_expect_tx(asked, 16);
                     ask_next_block(&answer, asked);
                 }
-                const bool answered = warp_wait(asked, a & 1, VOXQ_DEVERR_WAIT_FULL, maps.err);
+                const bool answered = warp_wait(asked, a & 1, VOXQ_DEVERR_WAIT_FULL, p.err);
                 ok = ok && answered;
                 if (!ok || !next_block(&answer, x, y, z)) break;
                 __syncwarp();
@@ -557,7 +543,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             int t0 = it.k_beg;
             float m = -INFINITY, l = 0.0f;  // m in base-2 units
             for (int i = 0; i < tiles; i++, t0 += kTcTile) {
-                ok = warp_wait(s_full + t, step++ & 1, VOXQ_DEVERR_WAIT_MMA, maps.err);
+                ok = warp_wait(s_full + t, step++ & 1, VOXQ_DEVERR_WAIT_MMA, p.err);
                 if (!ok) break;
                 tc_after();
                 uint32_t sv[kTcTile];
@@ -654,7 +640,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 for (int c = 0; c < HD; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + c));
             }
             if (ok && tiles > 0) {
-                ok = warp_wait(o_done + t, unit++ & 1, VOXQ_DEVERR_WAIT_MMA, maps.err);
+                ok = warp_wait(o_done + t, unit++ & 1, VOXQ_DEVERR_WAIT_MMA, p.err);
                 tc_after();
             }
             if (it.has(t)) {
@@ -738,11 +724,38 @@ static EncodeTiled encode_tiled() {
     return fn;
 }
 
+bool paged_maps_take(const voxq_paged_attn& d) {
+    const int64_t lim = (int64_t)1 << 38;  // elements: a tensor map's strides are below 2^40 bytes
+    return d.page_size > 0 && d.page_size % 8 == 0 && d.pages > 0 && d.page_stride > 0 && d.row_stride > 0 && d.head_stride > 0 &&
+           d.page_stride < lim && d.row_stride < lim && d.head_stride < lim;
+}
+
+VoxCPMError paged_maps(const voxq_paged_attn& d, int max_rows, PagedMaps* m) {
+    EncodeTiled enc = encode_tiled();
+    if (!enc) return VOXCPM_ERR_INTERNAL;
+    const int e = elem_bytes(d.dtype);
+    m->box_rows = d.page_size & -d.page_size;
+    if (m->box_rows > max_rows) m->box_rows = max_rows;
+    m->head_first = d.head_stride <= d.row_stride;
+    const int hi = m->head_first ? 1 : 2, ri = 3 - hi;
+    cuuint64_t dims[4] = {(cuuint64_t)d.head_dim, 0, 0, (cuuint64_t)d.pages}, strides[3] = {0, 0, (cuuint64_t)d.page_stride * e};
+    cuuint32_t box[4] = {(cuuint32_t)(128 / e), 1, 1, 1}, one[4] = {1, 1, 1, 1};
+    dims[hi] = (cuuint64_t)d.kv_heads;
+    dims[ri] = (cuuint64_t)d.page_size;
+    strides[hi - 1] = (cuuint64_t)d.head_stride * e;
+    strides[ri - 1] = (cuuint64_t)d.row_stride * e;
+    box[ri] = (cuuint32_t)m->box_rows;
+    const CUtensorMapDataType dt = d.dtype == VOXQ_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : d.dtype == VOXQ_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    for (int i = 0; i < 2; i++)
+        if (enc(i ? &m->v : &m->k, dt, 4, const_cast<void*>(i ? d.v : d.k), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return VOXCPM_ERR_UNSUPPORTED;
+    return VOXCPM_SUCCESS;
+}
+
 bool paged_tc_takes(const voxq_paged_attn& d) {
-    const int64_t lim = (int64_t)1 << 39;  // elements: a tensor map's strides are below 2^40 bytes
-    return d.dtype != VOXQ_F32 && (d.head_dim == 64 || d.head_dim == 128) && d.page_size > 0 && d.page_size % 8 == 0 && d.scale >= 0.0f &&
-           d.pages > 0 && d.page_stride > 0 && d.row_stride > 0 && d.head_stride > 0 && d.page_stride < lim && d.row_stride < lim &&
-           d.head_stride < lim;
+    return d.dtype != VOXQ_F32 && (d.head_dim == 64 || d.head_dim == 128) && d.scale >= 0.0f && paged_maps_take(d);
 }
 
 template <typename T, int HD>
@@ -753,26 +766,9 @@ static VoxCPMError tc_launch(const PagedArgs& a, cudaStream_t st) {
     std::call_once(once, [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem<HD>); });
     VOXQ_CUDA_TRY(attr);
     const voxq_paged_attn& d = a.d;
-    EncodeTiled enc = encode_tiled();
-    TcMaps m;
-    m.err = device_error_word();
-    if (!enc || !m.err) return VOXCPM_ERR_INTERNAL;
-    m.box_rows = d.page_size & -d.page_size;
-    if (m.box_rows > kTcTile) m.box_rows = kTcTile;
-    m.head_first = d.head_stride <= d.row_stride;
-    const int hi = m.head_first ? 1 : 2, ri = 3 - hi;
-    cuuint64_t dims[4] = {(cuuint64_t)HD, 0, 0, (cuuint64_t)d.pages}, strides[3] = {0, 0, (cuuint64_t)d.page_stride * 2};
-    cuuint32_t box[4] = {64, 1, 1, 1}, one[4] = {1, 1, 1, 1};
-    dims[hi] = (cuuint64_t)d.kv_heads;
-    dims[ri] = (cuuint64_t)d.page_size;
-    strides[hi - 1] = (cuuint64_t)d.head_stride * 2;
-    strides[ri - 1] = (cuuint64_t)d.row_stride * 2;
-    box[ri] = (cuuint32_t)m.box_rows;
-    const CUtensorMapDataType dt = std::is_same<T, bf16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    for (int i = 0; i < 2; i++)
-        if (enc(i ? &m.v : &m.k, dt, 4, const_cast<void*>(i ? d.v : d.k), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-            return VOXCPM_ERR_UNSUPPORTED;  // a layout that a tensor map cannot describe
+    PagedMaps m;
+    const VoxCPMError e = paged_maps(d, kTcTile, &m);
+    if (e != VOXCPM_SUCCESS) return e;
     const dim3 grid(((int)((int64_t)d.total_q * a.group / kTcRows) + d.batch) * d.kv_heads, 1, a.splits);
     VOXQ_CUDA_TRY(launch_pdl(kern, grid, dim3(kTcThreads), kTcSmem<HD>, st, a, m));
     return VOXCPM_SUCCESS;

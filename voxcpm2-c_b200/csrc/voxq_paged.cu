@@ -9,8 +9,6 @@
 
 namespace voxq {
 
-constexpr int kPagedThreads = 128;
-constexpr int kPagedMaxHeadDim = 256;
 constexpr int kSplitCtas = 4;   // CTAs per SM that splitting the keys aims at
 constexpr int kTcSplitCtas = 1;  // the same for the tcgen05 kernel, one CTA of which fills an SM
 constexpr int kTcMinRows = 64;   // rows a sequence from which that kernel's 128-row tiles pay
@@ -238,8 +236,15 @@ static PagedPlan paged_plan(const voxq_paged_attn& d) {
     PagedPlan r;
     const int G = d.heads / d.kv_heads;
     r.step = (int64_t)d.max_q * G <= 16 && paged_maps_take(d);
+    if (r.step) {
+        r.tc = false;
+        r.splits = 1;
+        r.split_len = INT32_MAX;
+        r.bytes = paged_step_bytes(d);
+        return r;
+    }
     r.tc = (int64_t)d.max_q * G > kTcMinRows && paged_tc_takes(d);
-    const int tr = r.tc ? kTcRows : r.step ? 16 : 64, ctas = r.tc ? kTcSplitCtas : kSplitCtas;
+    const int tr = r.tc ? kTcRows : 64, ctas = r.tc ? kTcSplitCtas : kSplitCtas;
     // CTAs without splitting, and the splits that bring them to kSplitCtas per SM
     const int64_t per_seq = std::max<int64_t>(1, std::min<int64_t>(d.batch, d.total_q));
     const int64_t tiles = std::max<int64_t>(per_seq, (int64_t)d.total_q * G / tr) * d.kv_heads;

@@ -21,6 +21,7 @@ struct PagedArgs {
     float2* ml;       // [total_q][heads][splits] running maximum and sum
     float* acc;       // [total_q][heads][splits][head_dim] unnormalised sums
     int* err;         // device error word of the bounded waits
+    int step_blocks, step_whole;  // voxq_paged_step.cu: blocks at most; no row's keys are cut
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -223,11 +224,14 @@ __device__ __forceinline__ void tma_page(uint32_t dst, const PagedMaps& m, const
                  : "memory");
 }
 
-// At most 16 rows a sequence (voxq_paged_step.cu); head_dim as any, caches that paged_maps_take.
+constexpr int kPagedThreads = 128;
+constexpr int kPagedMaxHeadDim = 256;
+// At most 16 rows a sequence (voxq_paged_step.cu), caches that paged_maps_take: everything that the call needs, and the
+// workspace that it takes.  VOXCPM_ERR_UNSUPPORTED, like paged_tc_launch, for a layout that a tensor map cannot describe.
+size_t paged_step_bytes(const voxq_paged_attn& d);
 VoxCPMError paged_step_launch(const PagedArgs& a, cudaStream_t st);
 // Attention on the tcgen05 tensor cores (voxq_paged_tc.cu): 16-bit types, head_dim 64 or 128, scale > 0, caches that
-// paged_maps_take.  Both launch the main kernel only and return VOXCPM_ERR_UNSUPPORTED for a layout that a tensor map
-// cannot describe.
+// paged_maps_take.  Launches the main kernel only.
 constexpr int kTcRows = 256;  // rows of a CTA
 bool paged_tc_takes(const voxq_paged_attn& d);
 VoxCPMError paged_tc_launch(const PagedArgs& a, cudaStream_t st);

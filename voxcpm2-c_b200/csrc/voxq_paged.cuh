@@ -10,6 +10,14 @@ namespace voxq {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// voxq_paged_step.cu: what a block leaves for the join of the row tile whose last piece it has.
+struct StepCut {
+    int pieces;           // its pieces, this block's and the ones before it; fewer than 2: nothing to join
+    int later;            // the first piece's block came to it after another part
+    int first, n, len;    // the sequence: first row in the batch, rows, positions
+    int row, kh;          // the tile's first row among n * group, kv head
+};
+
 // The call's sizes as the kernels take them.
 struct PagedArgs {
     voxq_paged_attn d;
@@ -21,6 +29,7 @@ struct PagedArgs {
     float2* ml;       // [total_q][heads][splits] running maximum and sum
     float* acc;       // [total_q][heads][splits][head_dim] unnormalised sums
     int* err;         // device error word of the bounded waits
+    StepCut* cut;     // voxq_paged_step.cu: [blocks]
     int step_blocks, step_whole;  // voxq_paged_step.cu: blocks at most; no row's keys are cut
 };
 

@@ -7,22 +7,24 @@
 
 namespace voxq {
 
-// Shape of the kernel: stages of 16 KB, SW for each consumer warp.
+constexpr int step_keys(int hd, int size) { return 8192 / (hd * size); }
+
+// Shape of the kernel: stages of 16 KB, SW for each warp.  (8 KB stages, two a warp: 39.4 us where this takes 38.0.)
 template <typename T, int HD>
 struct StepShape {
-    static constexpr int KT = 8192 / (HD * (int)sizeof(T));  // keys of a tile
+    static constexpr int KT = step_keys(HD, sizeof(T));      // keys of a tile
     static constexpr int BL = HD * (int)sizeof(T) / 128;     // 128-byte blocks of a row
     static constexpr int P = HD + 16 / (int)sizeof(T);       // shared pitch of the queries
-    static constexpr int W = 4, SW = 1, ST = W * SW;         // consumer warps, stages of each
+    static constexpr int W = 4, SW = 1, ST = W * SW;  // warps, stages of each
     static constexpr int stage = 2 * KT * HD * (int)sizeof(T);
     static constexpr int MP = HD + 4;                        // pitch of the warps' outputs while they are joined
     static constexpr int bytes = 1024 + ST * stage + W * 16 * MP * 4 + 16 * P * (int)sizeof(T);
     static constexpr int per_sm = HD > 128 ? 1 : 2;          // blocks that share an SM
     static_assert(per_sm * (bytes + 2048) <= 228 * 1024, "shared memory");
 };
-constexpr int kStepThreads = 160;
-constexpr int kWholeTiles = 16;   // a row's keys stay in one block up to here
-constexpr int kMinTiles = 8;      // tiles that are worth a block of their own
+constexpr int kStepThreads = 128;
+constexpr int kWholeTiles = 12;   // a row's keys stay in one block up to here
+constexpr int kMinTiles = 8;     // tiles that are worth a block of their own
 constexpr int kStepPieces = 512;  // most blocks, and so most pieces of one row
 
 // KT rows as 128-byte blocks of 128-byte-swizzled rows.
@@ -34,8 +36,6 @@ struct SwizzledRows {
         return base + (b / 128) * (KT * 128) + row * 128 + (((b % 128 / 16) ^ (row & 7)) << 4) + b % 16;
     }
 };
-
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // The work of a call as one line of key tiles: sequence by sequence, within it row tile by row tile (16 rows), kv head by
 // kv head, tile by tile.  The blocks take equal stretches of it, whatever the lengths are; a stretch that ends inside a
@@ -58,53 +58,28 @@ __device__ __forceinline__ StepSeq step_seq(const PagedArgs& p, int s) {
     q.units = (int64_t)((q.n * p.group + 15) / 16) * p.d.kv_heads * q.line;
     return q;
 }
-// Units before each thread's sequences tid * per .. and in total, over the block's THREADS threads.
-template <int THREADS, int KT>
-__device__ __forceinline__ int64_t step_scan(const PagedArgs& p, int per, int64_t& before) {
-    __shared__ int64_t sums[THREADS / 32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int64_t mine = 0;
-    for (int i = 0; i < per; i++) {
-        const int s = threadIdx.x * per + i;
-        if (s < p.d.batch) mine += step_seq<KT>(p, s).units;
-    }
-    int64_t run = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += v;
-    }
-    if (lane == 31) sums[warp] = run;
-    __syncthreads();
-    int64_t total = 0;
-    before = run - mine;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; w++) {
-        if (w < warp) before += sums[w];
-        total += sums[w];
-    }
-    return total;
-}
 __device__ __forceinline__ int step_blocks(const PagedArgs& p, int64_t total) {
     return (int)max((int64_t)1, min((int64_t)p.step_blocks, p.step_whole ? total : total / kMinTiles));
 }
 
 // Up to 16 rows -- pairs (token, query head of the kv head's group) -- against a sequence's keys: the next-token step.
 // It reads the cache once and computes little, so it is bound by HBM, by how early and how evenly the copies are issued
-// and by an even share for every block.  A producer warp does nothing but copy: its lanes look the pages of several
-// tiles' boxes up at once and issue their TMA copies, on into the next stretch of keys while the last is still at work;
-// boxes past the last key are left out.  (The same stages by cp.async, from this warp or from all, took 150 and 65 us
-// where this takes STEPUS for 64 sequences: a warp has few of those in flight.)  Each of four consumer warps takes every
-// fourth tile by itself, with its own running maximum m, sum l and outputs for the 16 rows, so no warp waits for another
-// until they are joined.  Two blocks share an SM: one's start and joins hide behind the other's stream.
+// and by an even share for every block.  Each of four warps takes every fourth tile of the block's stretch by itself, with
+// its own stages, running maximum m, sum l and outputs for the 16 rows, so no warp waits for another until they are
+// joined.  It also issues its own TMA copies, a lane per box of a page, SW tiles ahead and on into the next row's keys;
+// boxes past the last key are left out, and the pages of the tile after next are looked up meanwhile.  (One warp that
+// issues for all took 700 clocks a tile, most of them for the copies' operands, and was the bound of short calls; the
+// same stages by cp.async took 65 to 150 us where this takes 38 for 64 sequences of 600..4096 keys, 3.9 TB/s, since a warp has few of those in
+// flight.)  Two blocks share an SM: one's start and joins hide behind the other's stream.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kStepThreads, StepShape<T, HD>::per_sm) paged_step_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ PagedMaps maps) {
     using S = StepShape<T, HD>;
     constexpr int KT = S::KT, P = S::P, ST = S::ST, W = S::W, NB = HD / 8, KN = KT / 8, MP = S::MP;
     extern __shared__ uint8_t step_sh[];
-    __shared__ uint64_t full[ST], empty[ST];
+    __shared__ uint64_t full[ST];
     __shared__ float2 wml[W][16];
-    __shared__ int64_t start_base;
+    __shared__ int64_t sums[kStepThreads / 32], start_base;
+    __shared__ StepSeq start;
     __shared__ int start_seq;
     const uint32_t ring = (smem_u32(step_sh) + 1023) & ~1023u;
     float* mo = reinterpret_cast<float*>(step_sh + (ring - smem_u32(step_sh)) + ST * S::stage);
@@ -112,106 +87,146 @@ __global__ void __launch_bounds__(kStepThreads, StepShape<T, HD>::per_sm) paged_
     const voxq_paged_attn& d = p.d;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, G = p.group;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < ST; i++) {
-            mbar_init(full + i, 1);
-            mbar_init(empty + i, 1);
-        }
+        for (int i = 0; i < ST; i++) mbar_init(full + i, 1);
         mbar_fence_init();
     }
     pdl_wait();
     pdl_launch_dependents();
 
-    // this block's stretch [pos, end), and the sequence that it begins in
+    // This block's stretch [pos, end), and the sequence that it begins in: an inclusive scan of the sequences' steps.
     const int per = (d.batch + kStepThreads - 1) / kStepThreads;
-    int64_t before;
-    const int64_t total = step_scan<kStepThreads, KT>(p, per, before);
-    const int blocks = step_blocks(p, total);
-    if ((int)blockIdx.x >= blocks || total == 0) return;
-    int64_t pos = blockIdx.x * total / blocks;
-    const int64_t end = (blockIdx.x + 1) * total / blocks;
+    int64_t mine = 0;
     for (int i = 0; i < per; i++) {
         const int s = threadIdx.x * per + i;
-        if (s >= d.batch) break;
-        const int64_t units = step_seq<KT>(p, s).units;
-        if (pos >= before && pos < before + units) {
-            start_seq = s;
-            start_base = before;
-        }
-        before += units;
+        if (s < d.batch) mine += step_seq<KT>(p, s).units;
     }
+    int64_t before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+    }
+    if (lane == 31) sums[warp] = before;
     __syncthreads();
-    int s = start_seq;
-    int64_t base = start_base;
-
-    // Stage of the block's c-th tile: a warp has stages of its own, because a barrier's phases can only be told apart by
-    // who has seen each of them, and copies may land out of order.
-    auto slot_of = [](int c) { return c % W * S::SW + c / W % S::SW; };
-    // The part of the stretch at pos that lies in one item: tiles a .. b - 1 of row tile rt and kv head kh.
-    StepSeq q = step_seq<KT>(p, s);
-    int a, b, rt, kh;
-    auto part = [&] {
-        while (pos >= base + q.units) {
-            base += q.units;
-            q = step_seq<KT>(p, ++s);
-        }
-        const int64_t in = pos - base;
-        const int item = (int)(in / q.line);
-        a = (int)(in - (int64_t)item * q.line);
-        b = p.step_whole ? q.tiles : (int)min((int64_t)q.tiles, a + (end - pos));
-        kh = item % d.kv_heads;
-        rt = item / d.kv_heads;
-    };
-    auto past = [&] { return p.step_whole ? 1 : b - a; };
-    int c = 0;  // tiles before this part
-
-    if (warp == W) {
-        // A tile has `boxes` boxes: KT / R for each 128-byte block of its keys and values.  The lanes take as many tiles
-        // at a time as they have boxes for, and look the next ones' pages up before they wait for these ones' stages.
-        const int R = maps.box_rows, rows_per = KT / R, boxes = 2 * rows_per * S::BL, at_once = 32 / boxes;
-        const int mine = lane / boxes, box = lane % boxes, block = box / rows_per % S::BL, row = box % rows_per * R;
-        const bool value = box >= rows_per * S::BL;
-        bool ok = true;
-        for (; pos < end && ok; pos += past()) {
-            part();
-            const int32_t* table = d.block_table + s * d.table_stride;
-            const int k_stop = min(b * KT, q.len);
-            int page = 0, off = 0;
-            auto look_up = [&](int tile) {
-                const int key = tile * KT + row;
-                if (key >= k_stop) return;
-                const int e = p.page_shift >= 0 ? key >> p.page_shift : (int)((uint32_t)key / (uint32_t)d.page_size);
-                page = __ldg(table + e);
-                off = key - e * d.page_size;
-            };
-            look_up(a + mine);
-            for (int i = a; i < b && ok;) {
-                const int now_page = (uint32_t)page < (uint32_t)d.pages ? page : 0, now_off = off, from = i;
-                look_up(i + at_once + mine);
-                for (int u = 0; u < at_once && i < b; u++, i++, c++) {
-                    const int slot = slot_of(c);
-                    if (c >= ST) ok = __all_sync(0xffffffffu, mbar_wait_bounded(empty + slot, (c / ST - 1) & 1, VOXQ_DEVERR_WAIT_EMPTY, p.err));
-                    if (!ok) break;
-                    const bool live = from + mine == i && i * KT + row < k_stop;
-                    const int count = __popc(__ballot_sync(0xffffffffu, live));
-                    if (lane == 0) mbar_arrive_expect_tx(full + slot, count * R * 128);
-                    __syncwarp();
-                    if (live)
-                        tma_page(ring + slot * S::stage + (value ? S::stage / 2 : 0) + block * (KT * 128) + row * 128, maps,
-                                 value ? &maps.v : &maps.k, block * (128 / (int)sizeof(T)), now_off, kh, now_page, full + slot);
-                }
-            }
-        }
-        if (!ok)  // nothing of this block may still be writing its shared memory when it ends
-            for (int i = max(0, c - ST); i < c; i++) mbar_wait_bounded(full + slot_of(i), (i / ST) & 1, VOXQ_DEVERR_NONE, p.err);
+    before -= mine;
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < kStepThreads / 32; w++) {
+        if (w < warp) before += sums[w];
+        total += sums[w];
+    }
+    const int blocks = step_blocks(p, total);
+    if ((int)blockIdx.x >= blocks || total == 0) {
+        if (threadIdx.x == 0 && !p.step_whole) p.cut[blockIdx.x].pieces = 0;
         return;
     }
+    int64_t pos = blockIdx.x * total / blocks;
+    const int64_t end = (blockIdx.x + 1) * total / blocks;
+    if (pos >= before && pos < before + mine) {
+        int s = threadIdx.x * per;
+        StepSeq q = step_seq<KT>(p, s);
+        for (; pos >= before + q.units; q = step_seq<KT>(p, ++s)) before += q.units;
+        start = q;
+        start_seq = s;
+        start_base = before;
+    }
+    __syncthreads();
+    // A walk over the stretch: at pos, tiles a .. b - 1 of row tile rt and kv head kh of sequence s; c tiles before them.
+    struct Walk {
+        int64_t pos, base;
+        StepSeq q;
+        int s, a, b, rt, kh, c;
+    };
+    auto enter = [&](Walk& w) {
+        while (w.pos >= w.base + w.q.units) {
+            w.base += w.q.units;
+            w.q = step_seq<KT>(p, ++w.s);
+        }
+        const int64_t in = w.pos - w.base;
+        const int item = (int)(in / w.q.line);
+        w.a = (int)(in - (int64_t)item * w.q.line);
+        w.b = p.step_whole ? w.q.tiles : (int)min((int64_t)w.q.tiles, w.a + (end - w.pos));
+        w.kh = item % d.kv_heads;
+        w.rt = item / d.kv_heads;
+    };
+    auto leave = [&](Walk& w) {
+        w.c += w.b - w.a;
+        w.pos += p.step_whole ? 1 : w.b - w.a;
+    };
+    Walk it;
+    it.pos = pos;
+    it.base = start_base;
+    it.q = start;
+    it.s = start_seq;
+    it.c = 0;
+    enter(it);
 
+    // The warp's copies run ahead of its products with a walk of their own: its k-th tile, the block's 4 k + warp-th, goes
+    // to stage k % SW of its own.  (A barrier's phases can only be told apart by who has seen each of them, and copies may
+    // land out of order: stages that warps shared would be read too early.)  A lane has one of the tile's boxes: KT / R
+    // for each 128-byte block of its keys and values.
+    const int R = maps.box_rows, rows_per = KT / R, boxes = 2 * rows_per * S::BL;
+    const int block = lane / rows_per % S::BL, row_in = lane % rows_per * R;
+    const bool value = lane >= rows_per * S::BL;
+    const uint32_t box_at = ring + warp * S::SW * S::stage + (value ? S::stage / 2 : 0) + block * (KT * 128) + row_in * 128;
+    uint64_t* const bars = full + warp * S::SW;
+    Walk ahead = it;
+    int issued = 0, page = 0, off = 0;
+    bool more = true, live = false;
+    auto look_up = [&] {  // tile 4 issued + warp
+        const int x = issued * W + warp;
+        while (x >= ahead.c + ahead.b - ahead.a) {
+            leave(ahead);
+            more = ahead.pos < end;
+            if (!more) return;
+            enter(ahead);
+        }
+        const int key = (ahead.a + x - ahead.c) * KT + row_in;
+        live = lane < boxes && key < min(ahead.b * KT, ahead.q.len);
+        if (live) {
+            const int e = p.page_shift >= 0 ? key >> p.page_shift : (int)((uint32_t)key / (uint32_t)d.page_size);
+            page = __ldg(d.block_table + ahead.s * d.table_stride + e);
+            off = key - e * d.page_size;
+        }
+    };
+    auto issue = [&] {
+        if (!more) return;
+        const int k = issued % S::SW, count = __popc(__ballot_sync(0xffffffffu, live));
+        if (lane == 0) mbar_arrive_expect_tx(bars + k, count * R * 128);
+        __syncwarp();
+        if (live)
+            tma_page(box_at + k * S::stage, maps, value ? &maps.v : &maps.k, block * (128 / (int)sizeof(T)), off, ahead.kh,
+                     (uint32_t)page < (uint32_t)d.pages ? page : 0, bars + k);
+        issued++;
+        look_up();
+    };
+    look_up();
+#pragma unroll
+    for (int k = 0; k < S::SW; k++) issue();
+
+    // The block with the last piece of a cut item -- its first part, which does not begin the item but ends it -- notes
+    // what joining the pieces takes.
+    if (threadIdx.x == 0 && !p.step_whole) {
+        const int64_t at0 = pos - it.a;  // the item's first step
+        const int from = (int)(((at0 + 1) * blocks - 1) / total);
+        StepCut cut;
+        cut.pieces = it.a > 0 && it.b == it.q.tiles ? (int)blockIdx.x - from + 1 : 0;
+        cut.later = from * total / blocks < at0;
+        cut.first = it.q.first;
+        cut.n = it.q.n;
+        cut.len = it.q.len;
+        cut.row = it.rt * 16;
+        cut.kh = it.kh;
+        p.cut[blockIdx.x] = cut;
+    }
     constexpr int QC = HD * (int)sizeof(T) / 16;
     constexpr bool QREG = !is_f32<T> && HD <= 128;
     bool ok = true;
-    for (bool again = false; pos < end; pos += past(), again = true) {
-        part();
-        const int r0 = rt * 16, rows = min(q.n * G - r0, 16), k_stop = min(b * KT, q.len);
+    int done = 0;  // this warp's tiles
+    for (bool again = false; it.pos < end; again = true) {
+        if (again) enter(it);
+        const StepSeq q = it.q;
+        const int a = it.a, b = it.b, kh = it.kh, r0 = it.rt * 16, rows = min(q.n * G - r0, 16), k_stop = min(b * KT, q.len);
         // queries, and this lane's rows: g and g + 8
         for (int i = threadIdx.x; i < 16 * QC; i += 128) {
             const int r = i / QC, x = i % QC * (16 / (int)sizeof(T)), row = r0 + r;
@@ -220,7 +235,7 @@ __global__ void __launch_bounds__(kStepThreads, StepShape<T, HD>::per_sm) paged_
         }
         cp_async_commit();
         cp_async_wait<0>();
-        consumers_sync();
+        __syncthreads();
         uint32_t qf[QREG ? HD / 16 : 1][4];
         if constexpr (QREG) {
 #pragma unroll
@@ -236,11 +251,12 @@ __global__ void __launch_bounds__(kStepThreads, StepShape<T, HD>::per_sm) paged_
 #pragma unroll
         for (int j = 0; j < NB; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
         // (without keys there is one tile with nothing in it)
-        for (int i = a + ((warp - c) & (W - 1)); i < b && ok; i += W) {
-            const int x = c + i - a, slot = slot_of(x);
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(full + slot, (x / ST) & 1, VOXQ_DEVERR_WAIT_FULL, p.err));
+        for (int i = a + ((warp - it.c) & (W - 1)); i < b && ok; i += W) {
+            const int k = done % S::SW;
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(bars + k, (done / S::SW) & 1, VOXQ_DEVERR_WAIT_FULL, p.err));
             if (!ok) break;
-            const SwizzledRows<T, KT> ks{ring + slot * S::stage}, vs{ring + slot * S::stage + S::stage / 2};
+            const uint32_t at = ring + (warp * S::SW + k) * S::stage;
+            const SwizzledRows<T, KT> ks{at}, vs{at + S::stage / 2};
             const int valid = max(k_stop - i * KT, 0);
             if (valid < KT) {
                 // values past the last key may be anything, and 0 * NaN is NaN
@@ -252,9 +268,10 @@ __global__ void __launch_bounds__(kStepThreads, StepShape<T, HD>::per_sm) paged_
             }
             attend_keys<T, HD, KN>(p, qs, qf, ks, vs, i * KT + 2 * t, vis, m, l, o);
             __syncwarp();
-            if (lane == 0) mbar_arrive(empty + slot);
+            done++;
+            issue();
         }
-        c += b - a;
+        leave(it);
         // join the warps' shares of the keys
 #pragma unroll
         for (int e = 0; e < 2; e++) {
@@ -265,7 +282,7 @@ __global__ void __launch_bounds__(kStepThreads, StepShape<T, HD>::per_sm) paged_
             for (int j = 0; j < NB; j++)
                 *reinterpret_cast<float2*>(mo + (warp * 16 + g + 8 * e) * MP + j * 8 + 2 * t) = make_float2(o[j][2 * e], o[j][2 * e + 1]);
         }
-        consumers_sync();
+        __syncthreads();
         const int r = threadIdx.x >> 3, row = r0 + r;  // 8 threads a row
         if (r < rows && ok) {
             float mm = -INFINITY, ll = 0.0f, f[W];
@@ -294,47 +311,28 @@ __global__ void __launch_bounds__(kStepThreads, StepShape<T, HD>::per_sm) paged_
                 else *reinterpret_cast<float2*>(p.acc + rec * d.head_dim + x) = v;
             }
         }
-        consumers_sync();  // the joined outputs and the queries are read
+        __syncthreads();  // the joined outputs and the queries are read
     }
+    if (!ok)  // nothing of this block may still be writing its shared memory when it ends
+        for (; done < issued; done++) mbar_wait_bounded(bars + done % S::SW, (done / S::SW) & 1, VOXQ_DEVERR_NONE, p.err);
 }
 
 // Joins the pieces of a row that several blocks worked on, in their order: M = max m, out = sum acc 2^(m - M) / sum l 2^(m - M).
-// One CTA per token and query head, its warps along the pieces.
-template <typename T, int KT>
+// One CTA for each block of the attention and row of its first part, its warps along the pieces; most have nothing to do.
+template <typename T>
 __global__ void __launch_bounds__(kPagedThreads) step_combine_kernel(const __grid_constant__ PagedArgs p) {
     constexpr int W = kPagedThreads / 32, PER = kStepPieces / kPagedThreads;
     __shared__ float weight[kStepPieces];
     __shared__ __align__(16) float part[W][kPagedMaxHeadDim];
     __shared__ float red[2][W];
-    __shared__ int64_t seq_base;
     const voxq_paged_attn& d = p.d;
-    const int tok = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.group;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.group;
     pdl_wait();
     pdl_launch_dependents();
-    const int per = (d.batch + kPagedThreads - 1) / kPagedThreads;
-    int64_t before;
-    const int64_t total = step_scan<kPagedThreads, KT>(p, per, before);
-    int s = -1;
-    for (int i0 = 0; i0 < d.batch; i0 += kPagedThreads) {
-        const int i = i0 + threadIdx.x;
-        s += __syncthreads_count(i < d.batch && __ldg(d.cu_q + i) <= tok);
-    }
-    s = max(s, 0);
-    if (s / per == (int)threadIdx.x) {
-        for (int i = threadIdx.x * per; i < s; i++) before += step_seq<KT>(p, i).units;
-        seq_base = before;
-    }
-    __syncthreads();
-    const StepSeq q = step_seq<KT>(p, s);
-    if (tok < q.first || tok >= q.first + q.n) return;
-    // the row's tiles, and the blocks a .. b that worked on them: block x has [x total / blocks, (x + 1) total / blocks)
-    const int blocks = step_blocks(p, total), row = (tok - q.first) * G + h % G;
-    const int64_t at0 = seq_base + ((int64_t)(row / 16) * d.kv_heads + h / G) * q.tiles;
-    auto owner = [&](int64_t x) { return (int)(((x + 1) * blocks - 1) / total); };
-    const int a = owner(at0), b = owner(at0 + q.tiles - 1), z = b - a + 1;
-    if (z == 1) return;
-    const int later = a * total / blocks < at0 ? 1 : 0;  // the first of them came to this row after another
-    auto record = [&](int j) { return (int64_t)((a + j) * 2 + (j == 0 ? later : 0)) * 16 + row % 16; };
+    const StepCut cut = p.cut[blockIdx.x];
+    const int z = cut.pieces, row = cut.row + blockIdx.y, a = blockIdx.x - z + 1;
+    if (z < 2 || row >= cut.n * G) return;
+    auto record = [&](int j) { return (int64_t)((a + j) * 2 + (j == 0 ? cut.later : 0)) * 16 + blockIdx.y; };
     float2 ml[PER];
     float m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -377,8 +375,8 @@ __global__ void __launch_bounds__(kPagedThreads) step_combine_kernel(const __gri
         *reinterpret_cast<float4*>(&part[warp][c]) = v;
     }
     __syncthreads();
-    const float inv = visible(p, q.len, q.n, tok - q.first) > 0 ? 1.0f / l : 0.0f;
-    const int64_t at = tok * d.o_stride + h * d.o_head_stride;
+    const float inv = visible(p, cut.len, cut.n, row / G) > 0 ? 1.0f / l : 0.0f;
+    const int64_t at = (cut.first + row / G) * d.o_stride + (cut.kh * G + row % G) * d.o_head_stride;
     for (int c = threadIdx.x * 2; c < d.head_dim; c += 2 * kPagedThreads) {
         float x = 0.0f, y = 0.0f;
 #pragma unroll
@@ -390,13 +388,8 @@ __global__ void __launch_bounds__(kPagedThreads) step_combine_kernel(const __gri
     }
 }
 
-static int step_keys(const voxq_paged_attn& d) {  // StepShape's KT
-    const int hd = d.head_dim <= 64 ? 64 : d.head_dim <= 128 ? 128 : 256;
-    return 8192 / (hd * elem_bytes(d.dtype));
-}
-
 int paged_step_blocks(const voxq_paged_attn& d, int* whole) {
-    const int kt = step_keys(d), group = d.heads / d.kv_heads;
+    const int kt = step_keys(d.head_dim <= 64 ? 64 : d.head_dim <= 128 ? 128 : 256, elem_bytes(d.dtype)), group = d.heads / d.kv_heads;
     // as many items and tiles as the bounds admit
     const int64_t items = ((int64_t)d.total_q * group / 16 + std::min(d.batch, d.total_q)) * d.kv_heads;
     const int64_t tiles = std::max<int64_t>((d.max_kv + (int64_t)kt - 1) / kt, 1);
@@ -408,7 +401,7 @@ int paged_step_blocks(const voxq_paged_attn& d, int* whole) {
 size_t paged_step_bytes(const voxq_paged_attn& d) {
     int whole;
     const int blocks = paged_step_blocks(d, &whole);
-    return whole ? 0 : (size_t)blocks * 2 * 16 * (8 + 4 * (size_t)d.head_dim);
+    return whole ? 0 : (size_t)blocks * (2 * 16 * (8 + 4 * (size_t)d.head_dim) + sizeof(StepCut));
 }
 
 template <typename T, int HD>
@@ -424,7 +417,7 @@ static VoxCPMError step_launch(const PagedArgs& a, cudaStream_t st) {
     if (e != VOXCPM_SUCCESS) return e;
     VOXQ_CUDA_TRY(launch_pdl(kern, dim3(a.step_blocks), dim3(kStepThreads), S::bytes, st, a, m));
     if (!a.step_whole)
-        VOXQ_CUDA_TRY(launch_pdl(step_combine_kernel<T, S::KT>, dim3(a.d.total_q, a.d.heads), dim3(kPagedThreads), 0, st, a));
+        VOXQ_CUDA_TRY(launch_pdl(step_combine_kernel<T>, dim3(a.step_blocks, std::min<int64_t>(16, (int64_t)a.d.max_q * a.group)), dim3(kPagedThreads), 0, st, a));
     return VOXCPM_SUCCESS;
 }
 
@@ -433,6 +426,7 @@ VoxCPMError paged_step_launch(const PagedArgs& call, cudaStream_t st) {
     a.step_blocks = paged_step_blocks(a.d, &a.step_whole);
     a.acc = (float*)a.d.workspace;
     a.ml = (float2*)(a.acc + (size_t)a.step_blocks * 2 * 16 * a.d.head_dim);
+    a.cut = (StepCut*)(a.ml + (size_t)a.step_blocks * 2 * 16);
     return with_elem(a.d.dtype, [&](auto x) {
         using T = decltype(x);
         const int hd = a.d.head_dim;

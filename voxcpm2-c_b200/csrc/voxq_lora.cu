@@ -16,25 +16,23 @@ template <typename T, typename W, int TM>
 struct LoraShape {
     static constexpr int WM = TM / 16;                // warps along the rows
     static constexpr int WK = kLoraWarps / WM;        // warps along K (first product) or the columns (second)
-    static constexpr int KB = is_f32<W> || (is_f32<T> && TM == 64) ? 64 : 128;  // K per stage (two fit in shared memory)
+    static constexpr int KB = is_f32<W> || TM == 64 ? 64 : 128;  // K per stage: four blocks of TM 64 share an SM
     static constexpr int NB = TM == 64 ? 64 : 128;    // output columns per step
     static constexpr int NW = NB / WK;                // of a warp
     static constexpr int XP = KB + 16 / sizeof(T);    // shared pitches: 16 bytes more than a row, so that the 8 rows
     static constexpr int AP = KB + 16 / sizeof(W);    // of a fragment load lie in different banks
-    static constexpr int OP = NW + 4;
     int Rp, stage, hp, bp;                            // rank in steps of 16; bytes of a stage; pitches of h and B
-    int o_hpart, o_hs, o_b0, o_b1, o_out, bytes;      // byte offsets
+    int o_hpart, o_hs, o_b0, o_b1, bytes;      // byte offsets
     __host__ __device__ explicit LoraShape(int rank) {
         Rp = (rank + 15) / 16 * 16;
         stage = TM * XP * (int)sizeof(T) + Rp * AP * (int)sizeof(W);
         hp = Rp + 8;
         bp = Rp + 16 / (int)sizeof(W);
         // the stages are free once the first product is done: the second
-        // buffer of B and the output staging live there
-        const int bbytes = NB * bp * (int)sizeof(W), obytes = kLoraWarps * 16 * OP * 4;
+        // buffer of B lives there
+        const int bbytes = NB * bp * (int)sizeof(W);
         o_b1 = 0;
-        o_out = bbytes;
-        const int low = 2 * stage > bbytes + obytes ? 2 * stage : bbytes + obytes;
+        const int low = 2 * stage > bbytes ? 2 * stage : bbytes;
         o_hpart = (low + 15) / 16 * 16;
         o_hs = o_hpart + WK * TM * hp * 4;
         o_b0 = o_hs + TM * hp * 4;  // fp32, or two 16-bit parts
@@ -89,16 +87,19 @@ __device__ __forceinline__ void mul_16(float (*d)[4], const T* as, const T* as_l
     }
 }
 
-// NW columns of B[w] from n0 on, [column][rank], to shared memory; zeros past
-// N and past the adapter's own rank r (what lies there may be anything).
-template <typename W, int NB>
-__device__ __forceinline__ void load_b(W* dst, int bp, const W* b, int n0, int N, int rank, int r, int Rp) {
+// NB columns of B[w] from n0 on, [column][rank], to shared memory; zeros past N and past the adapter's own rank r (what
+// lies there may be anything).  Within a warp's NW columns, column c goes to row (c % CW / 2) * 8 + 2 (c / CW) + c % 2
+// with CW = NW / 4: the columns that a thread gets from the MMAs -- 2 t and 2 t + 1 of every block of 8 rows -- are then
+// CW neighbours of the output, and base and out move straight between memory and the accumulators.  per: 16-byte vectors of a column, inv: 2^20 / per rounded up.
+template <typename W, int NB, int NW>
+__device__ __forceinline__ void load_b(W* dst, int bp, const W* b, int n0, int N, int rank, int r, int per, uint32_t inv) {
     constexpr int E = 16 / sizeof(W);
-    const int per = Rp / E;
     for (int i = threadIdx.x; i < NB * per; i += kLoraThreads) {
-        const int row = i / per, c = (i - row * per) * E;
+        constexpr int CW = NW / 4;
+        const int row = (uint32_t)i * inv >> 20, c = (i - row * per) * E, in = row % NW;
+        const int to = row - in + in % CW / 2 * 8 + in / CW * 2 + in % 2;
         const bool ok = n0 + row < N && c < r;
-        const W* src = b + (int64_t)(ok ? n0 + row : 0) * rank + (ok ? c : 0);
+        const W* src = b + (ok ? (int64_t)(n0 + row) * rank + c : 0);
         if (ok && c + E > r) {  // the adapter's rank ends inside these 16 bytes
             uint4 v = *reinterpret_cast<const uint4*>(src);
             W e[E];
@@ -107,9 +108,9 @@ __device__ __forceinline__ void load_b(W* dst, int bp, const W* b, int n0, int N
             for (int j = 0; j < E; j++)
                 if (c + j >= r) e[j] = from_f<W>(0.0f);
             memcpy(&v, e, 16);
-            *reinterpret_cast<uint4*>(dst + row * bp + c) = v;
+            *reinterpret_cast<uint4*>(dst + to * bp + c) = v;
         } else {
-            cp_async16_or_zero(dst + row * bp + c, src, ok);
+            cp_async16_or_zero(dst + to * bp + c, src, ok);
         }
     }
 }
@@ -150,28 +151,38 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
     const W* wa = (const W*)d.a + (int64_t)w * d.rank * d.K;
     const W* wb = (const W*)d.b + (int64_t)w * d.N * d.rank;
     const int blocks = (r + 7) / 8, inner = (r + 15) / 16;
+    const int per = z.Rp / (16 / (int)sizeof(W));
+    const uint32_t inv = (1u << 20) / per + 1;
 
     W* bs0 = reinterpret_cast<W*>(lora_sh + z.o_b0);
     T* hs = reinterpret_cast<T*>(lora_sh + z.o_hs);  // h as two 16-bit parts, or fp32
     T* hs_lo = hs + (is_f32<T> ? 0 : TM * z.hp);
     if (r > 0) {
-        load_b<W, NB>(bs0, z.bp, wb, crank * NB, d.N, d.rank, r, z.Rp);
+        load_b<W, NB, NW>(bs0, z.bp, wb, crank * NB, d.N, d.rank, r, per, inv);
         cp_async_commit();
         const int chunks = (d.K + KB - 1) / KB, mine = chunks > (int)crank ? (chunks - crank + csize - 1) / csize : 0;
+        // A chunk of K to its stage.  Rows of x past the tile's and of A past the rank keep what was there: they only reach
+        // sums that nobody reads.
+        constexpr int EX = 16 / sizeof(T), EA = 16 / sizeof(W), VX = KB / EX, VA = KB / EA, RX = kLoraThreads / VX, RA = kLoraThreads / VA;
+        const int rx = threadIdx.x / VX, kx = threadIdx.x % VX * EX, ra = threadIdx.x / VA, ka = threadIdx.x % VA * EA;
+        const T* x0 = (const T*)d.x + (m0 + rx) * d.ldx + kx;
+        const W* a0 = wa + (int64_t)ra * d.K + ka;
         auto fetch = [&](int c) {
             T* xs = reinterpret_cast<T*>(lora_sh + (c & 1) * z.stage);
             W* as = reinterpret_cast<W*>(xs + TM * S::XP);
             const int k0 = (crank + c * csize) * KB;
-            constexpr int EX = 16 / sizeof(T), EA = 16 / sizeof(W);
-            for (int i = threadIdx.x; i < TM * (KB / EX); i += kLoraThreads) {
-                const int row = i / (KB / EX), col = i % (KB / EX) * EX;
-                const bool ok = row < rows && k0 + col < d.K;
-                cp_async16_or_zero(xs + row * S::XP + col, (const T*)d.x + (ok ? (m0 + row) * d.ldx + k0 + col : 0), ok);
+            const bool okx = k0 + kx < d.K, oka = k0 + ka < d.K;
+            const T* xp = okx ? x0 + k0 : (const T*)d.x;
+            const W* ap = oka ? a0 + k0 : wa;
+#pragma unroll 2
+            for (int row = rx; row < rows; row += RX) {
+                cp_async16_or_zero(xs + row * S::XP + kx, xp, okx);
+                xp += okx ? RX * d.ldx : 0;
             }
-            for (int i = threadIdx.x; i < z.Rp * (KB / EA); i += kLoraThreads) {
-                const int row = i / (KB / EA), col = i % (KB / EA) * EA;
-                const bool ok = row < r && k0 + col < d.K;
-                cp_async16_or_zero(as + row * S::AP + col, wa + (ok ? (int64_t)row * d.K + k0 + col : 0), ok);
+#pragma unroll 2
+            for (int row = ra; row < r; row += RA) {
+                cp_async16_or_zero(as + row * S::AP + ka, ap, oka);
+                ap += oka ? (int64_t)RA * d.K : 0;
             }
         };
         float acc[RB][4];
@@ -238,65 +249,59 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     }
 
-    // Columns n0 .. n0 + NB - 1 at a time; a warp owns 16 rows x NW columns of
-    // them and turns its fragments into rows through its own staging, so that
-    // base and out move in 16-byte accesses.
-    constexpr int E = 16 / sizeof(T), PER = 16 * NW / E / 32;
-    float* ost = reinterpret_cast<float*>(lora_sh + z.o_out) + warp * 16 * S::OP;
+    // Columns n0 .. n0 + NB - 1 at a time; a warp owns 16 rows x NW columns of them, a thread CW neighbours of rows g and
+    // g + 8.  base comes a step ahead.
+    constexpr int E = 16 / sizeof(T), CW = NW / 4, VC = CW / E;  // vectors of a row
     W* bs1 = reinterpret_cast<W*>(lora_sh + z.o_b1);
-    const int step = csize * NB;
+    const int step = csize * NB, g = lane >> 2, c0 = (WK > 1 ? wk * NW : 0) + (lane & 3) * CW, row0 = wm * 16 + g;
+    const T* base0 = (const T*)d.base + (m0 + row0) * d.ldb + c0;
+    T* out0 = (T*)d.out + (m0 + row0) * d.ldo + c0;
+    auto fetch_base = [&](int n0, uint4 (&v)[2][VC]) {
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int j = 0; j < VC; j++) {
+                v[e][j] = make_uint4(0, 0, 0, 0);
+                if (d.base && row0 + 8 * e < rows && n0 + c0 + j * E < d.N)
+                    v[e][j] = *reinterpret_cast<const uint4*>(base0 + 8 * e * d.ldb + n0 + j * E);
+            }
+    };
+    uint4 old[2][VC], next[2][VC];
+    fetch_base(crank * NB, old);
     int it = 0;
     for (int n0 = crank * NB; n0 < d.N; n0 += step, it++) {
-        const int nw = n0 + (WK > 1 ? wk * NW : 0);
-        uint4 old[PER];
-        bool ok[PER];
+        fetch_base(n0 + step, next);
+        float o[NW / 8][4];
 #pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const int i = lane + 32 * j, row = wm * 16 + i / (NW / E), col = nw + i % (NW / E) * E;
-            ok[j] = row < rows && col < d.N;
-            old[j] = make_uint4(0, 0, 0, 0);
-            if (ok[j] && d.base) old[j] = *reinterpret_cast<const uint4*>((const T*)d.base + (m0 + row) * d.ldb + col);
-        }
+        for (int i = 0; i < NW / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
         if (r > 0) {
             cp_async_wait<0>();
             __syncthreads();  // this step's B has landed (and h is written); the other buffer is free
-            if (n0 + step < d.N) load_b<W, NB>(it & 1 ? bs0 : bs1, z.bp, wb, n0 + step, d.N, d.rank, r, z.Rp);
+            if (n0 + step < d.N) load_b<W, NB, NW>(it & 1 ? bs0 : bs1, z.bp, wb, n0 + step, d.N, d.rank, r, per, inv);
             cp_async_commit();
             const W* bs = (it & 1 ? bs1 : bs0) + (WK > 1 ? wk * NW * z.bp : 0);
-            float o[NW / 8][4];
-#pragma unroll
-            for (int i = 0; i < NW / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
             for (int k = 0; k < inner; k++)
                 mul_16<T, W, NW / 8, !is_f32<T>>(o, hs + wm * 16 * z.hp + k * 16, hs_lo + wm * 16 * z.hp + k * 16, z.hp,
                                                  bs + k * 16, z.bp, NW / 8);
-            const int g = lane >> 2, t = lane & 3;
-            __syncwarp();  // the last step's rows are read
-#pragma unroll
-            for (int i = 0; i < NW / 8; i++) {
-                *reinterpret_cast<float2*>(ost + g * S::OP + i * 8 + 2 * t) = make_float2(o[i][0], o[i][1]);
-                *reinterpret_cast<float2*>(ost + (g + 8) * S::OP + i * 8 + 2 * t) = make_float2(o[i][2], o[i][3]);
-            }
-            __syncwarp();
         }
 #pragma unroll
-        for (int j = 0; j < PER; j++) {
-            if (!ok[j]) continue;
-            const int i = lane + 32 * j, lr = i / (NW / E), lc = i % (NW / E) * E;
-            if (r > 0) {
-                T e[E];
-                memcpy(e, &old[j], 16);
+        for (int e = 0; e < 2; e++)
 #pragma unroll
-                for (int v = 0; v < E; v += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(ost + lr * S::OP + lc + v);
-                    e[v] = from_f<T>(to_f(e[v]) + f.x);
-                    e[v + 1] = from_f<T>(to_f(e[v + 1]) + f.y);
-                    e[v + 2] = from_f<T>(to_f(e[v + 2]) + f.z);
-                    e[v + 3] = from_f<T>(to_f(e[v + 3]) + f.w);
+            for (int j = 0; j < VC; j++) {
+                if (row0 + 8 * e >= rows || n0 + c0 + j * E >= d.N) continue;
+                if (r > 0) {
+                    T x[E];
+                    memcpy(x, &old[e][j], 16);
+#pragma unroll
+                    for (int v = 0; v < E; v++) x[v] = from_f<T>(to_f(x[v]) + o[(j * E + v) / 2][2 * e + v % 2]);
+                    memcpy(&old[e][j], x, 16);
                 }
-                memcpy(&old[j], e, 16);
+                *reinterpret_cast<uint4*>(out0 + 8 * e * d.ldo + n0 + j * E) = old[e][j];
             }
-            *reinterpret_cast<uint4*>((T*)d.out + (m0 + wm * 16 + lr) * d.ldo + nw + lc) = old[j];
-        }
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int j = 0; j < VC; j++) old[e][j] = next[e][j];
     }
     cp_async_wait<0>();
     if (r > 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");

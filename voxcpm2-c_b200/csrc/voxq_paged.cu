@@ -162,8 +162,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_combine_kernel(const __gr
     __shared__ float red[2][W];
     const voxq_paged_attn& d = p.d;
     const int tok = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    pdl_wait();
-    pdl_launch_dependents();
+    // (the batch's integers were complete before the attention let this kernel start)
     int s = -1;
     for (int i0 = 0; i0 < d.batch; i0 += kPagedThreads) {
         const int i = i0 + threadIdx.x;
@@ -173,6 +172,8 @@ __global__ void __launch_bounds__(kPagedThreads) paged_combine_kernel(const __gr
     const int first = __ldg(d.cu_q + s), n = min(__ldg(d.cu_q + s + 1), d.total_q) - first;
     const int len = min(max(__ldg(d.kv_len + s), 0), d.max_kv);
     const int seen = tok >= first && tok < first + n ? visible(p, len, n, tok - first) : 0;
+    pdl_wait();
+    pdl_launch_dependents();
     if (seen <= p.split_len) return;
     const int z = (seen + p.split_len - 1) / p.split_len;
     const int64_t rec = ((int64_t)tok * d.heads + h) * p.splits;
@@ -245,10 +246,10 @@ static PagedPlan paged_plan(const voxq_paged_attn& d) {
     }
     r.tc = (int64_t)d.max_q * G > kTcMinRows && paged_tc_takes(d);
     const int tr = r.tc ? kTcRows : 64, ctas = r.tc ? kTcSplitCtas : kSplitCtas;
-    // CTAs without splitting, and the splits that bring them to kSplitCtas per SM
-    const int64_t per_seq = std::max<int64_t>(1, std::min<int64_t>(d.batch, d.total_q));
-    const int64_t tiles = std::max<int64_t>(per_seq, (int64_t)d.total_q * G / tr) * d.kv_heads;
-    const int64_t want = (ctas * device_sm_count() + tiles - 1) / tiles;
+    // CTAs without splitting (at most one more than full tiles for every sequence), and the splits that bring them to
+    // `ctas` an SM without a second round
+    const int64_t tiles = ((int64_t)d.total_q * G / tr + std::min(d.batch, d.total_q)) * d.kv_heads;
+    const int64_t want = std::max<int64_t>(1, ctas * device_sm_count() / tiles);
     const int64_t most = std::max<int64_t>(1, (d.max_kv + kMinSplit - 1) / kMinSplit);
     const int64_t z = std::min(std::min(want, most), (int64_t)kMaxSplits);
     r.split_len = (int)(((d.max_kv + z - 1) / z + 127) / 128 * 128);  // whole tiles of either kernel

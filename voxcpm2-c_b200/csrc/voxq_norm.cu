@@ -73,7 +73,7 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 // rows, by the latency of one load and two reductions for a few.  WR warps
 // hold a whole row in registers, PER vectors of V elements a thread, so the
 // second norm needs no second read; all of a row's loads are issued before the
-// first reduction, and with one warp per row no block barrier is needed.
+// first reduction.
 // h stays fp32 from its sum to the norm.
 template <typename T, int V, int WR, int PER>
 __global__ void __launch_bounds__(WR == 1 ? 128 : 32 * WR) norm_residual_kernel(const __grid_constant__ voxq_norm d) {
@@ -157,28 +157,22 @@ static cudaError_t norm_launch(const voxq_norm& d, cudaStream_t st) {
     return launch_pdl(norm_residual_kernel<T, V, WR, PER>, dim3(blocks), dim3(WR == 1 ? 128 : 32 * WR), 0, st, d);
 }
 
-// Warps per row: as few as hold it in 8 vectors a thread when there are rows
-// enough to fill the GPU (no block barrier, most bytes in flight per thread),
-// else as many as leave 2 (shorter chains per thread).
+// One vector a thread as far as 512 threads go: the shortest chains and the most rows in flight.  (8191 rows of 1024 in
+// bf16, gated, with both norms: 24.6 us from cold caches with 4 warps of one vector a row, 26.6 with one warp of four,
+// 28.7 with 4 warps and room for two.)
 template <typename T>
 static cudaError_t norm_dispatch(const voxq_norm& d, bool wide, cudaStream_t st) {
     constexpr int V = 16 / sizeof(T);
     if (!wide)  // odd widths and alignments, one element per access
         return d.D <= 1024 ? norm_launch<T, 1, 4, 8>(d, st) : norm_launch<T, 1, 16, 32>(d, st);
     const int nv = d.D / V;
-    const bool few = d.rows < 8 * device_sm_count();
-    if (nv <= (few ? 64 : 256)) {
-        if (nv <= 64) return norm_launch<T, V, 1, 2>(d, st);
-        else if (nv <= 128) return norm_launch<T, V, 1, 4>(d, st);
-        else return norm_launch<T, V, 1, 8>(d, st);
-    } else if (nv <= (few ? 256 : 1024)) {
-        if (nv <= 256) return norm_launch<T, V, 4, 2>(d, st);
-        else return norm_launch<T, V, 4, 8>(d, st);
-    } else if (nv <= 1024) {
-        return norm_launch<T, V, 16, 2>(d, st);
-    } else {
-        return norm_launch<T, V, 16, 8>(d, st);
-    }
+    if (nv <= 32) return norm_launch<T, V, 1, 1>(d, st);
+    if (nv <= 64) return norm_launch<T, V, 2, 1>(d, st);
+    if (nv <= 128) return norm_launch<T, V, 4, 1>(d, st);
+    if (nv <= 256) return norm_launch<T, V, 8, 1>(d, st);
+    if (nv <= 512) return norm_launch<T, V, 16, 1>(d, st);
+    if (nv <= 1024) return norm_launch<T, V, 16, 2>(d, st);
+    return norm_launch<T, V, 16, 8>(d, st);
 }
 
 }  // namespace voxq

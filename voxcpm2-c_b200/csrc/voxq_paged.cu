@@ -15,6 +15,8 @@ constexpr int kTcMinRows = 64;   // rows a sequence from which that kernel's 128
 constexpr int kMinSplit = 256;  // keys that are worth a CTA of their own
 constexpr int kMaxSplits = 128;
 
+constexpr int kMmaThreads = 256;
+
 // Shape of the kernel for element type T and head dims up to HD.
 template <typename T, int HD>
 struct PagedShape {
@@ -23,29 +25,31 @@ struct PagedShape {
     static constexpr int ST = HD > 128 ? 2 : 3;            // cp.async stages
     static constexpr int P = HD + 16 / (int)sizeof(T);     // shared pitch: 16 bytes more than a row
     static constexpr int stage = 2 * BK * P * (int)sizeof(T);
+    static constexpr int MP = HD + 4;                      // pitch of the rows' sums while the two halves are joined
     static constexpr int bytes = TR * P * (int)sizeof(T) + ST * stage;
-    static_assert(bytes <= 227 * 1024, "shared memory");
+    static_assert(bytes <= 227 * 1024 && TR * MP * 4 <= ST * stage, "shared memory");
 };
 
 // Attention of more than 16 rows a sequence on warp-level MMAs: fp32, and the head dims and page sizes that the tcgen05
 // kernel does not take; and any number of rows where a tensor map cannot describe the caches.
 //
 // The rows of a tile are the pairs (token, query head of the kv head's group), so a key is read once for all heads that
-// share it; each of the four warps owns 16 rows and all keys of a tile.  Keys and values of BK positions arrive by
+// share it.  Two warps own each 16 rows and take half of a tile's keys each, with their own maximum and sums, joined at the
+// end: a lone warp on a quarter of an SM waits for its own MMAs.  Keys and values of BK positions arrive by
 // cp.async, three stages deep, each thread following the block table for its own rows of the tile (a page may end
 // anywhere inside it); rows past the end are zeros in shared memory, whatever the cache holds.  One pass, base-2 softmax
 // with running maximum m and sum l per row.  With few tiles the keys are split over CTAs (blockIdx.z); a row with more
 // than one split leaves (m, l, sums) for paged_combine_kernel.
 template <typename T, int HD>
-__global__ void __launch_bounds__(kPagedThreads) paged_mma_kernel(const __grid_constant__ PagedArgs p) {
+__global__ void __launch_bounds__(kMmaThreads) paged_mma_kernel(const __grid_constant__ PagedArgs p) {
     using S = PagedShape<T, HD>;
-    constexpr int TR = S::TR, BK = S::BK, P = S::P, ST = S::ST, NB = HD / 8;
+    constexpr int TR = S::TR, BK = S::BK, P = S::P, ST = S::ST, NB = HD / 8, KW = BK / 2;  // keys of a warp
     extern __shared__ __align__(16) uint8_t paged_sh[];
     T* qs = reinterpret_cast<T*>(paged_sh);
     T* kv = qs + TR * P;
     const voxq_paged_attn& d = p.d;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int kh = blockIdx.y, G = p.group;
+    const int wm = warp & 3, wk = warp >> 2, kh = blockIdx.y, G = p.group;
     pdl_wait();
     pdl_launch_dependents();
     const int s = tile_owner<TR>(d.cu_q, d.batch, G, blockIdx.x);
@@ -58,7 +62,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_mma_kernel(const __grid_c
     if (k_beg >= k_end && blockIdx.z > 0) return;
     const int32_t* table = d.block_table + s * d.table_stride;
 
-    constexpr int E = 16 / sizeof(T), CPR = HD / E, RP = kPagedThreads / CPR;  // vectors per row, rows per pass
+    constexpr int E = 16 / sizeof(T), CPR = HD / E, RP = kMmaThreads / CPR;  // vectors per row, rows per pass
     const int lc = threadIdx.x % CPR * E, lr = threadIdx.x / CPR;
     auto fetch = [&](int t0, int stage) {
         T* ks = kv + stage * 2 * BK * P + lr * P + lc;
@@ -75,7 +79,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_mma_kernel(const __grid_c
             cp_async16_or_zero(ks + (BK + j * RP) * P, (const T*)d.v + o, at[j] >= 0);
         }
     };
-    for (int i = threadIdx.x; i < TR * CPR; i += kPagedThreads) {
+    for (int i = threadIdx.x; i < TR * CPR; i += kMmaThreads) {
         const int r = i / CPR, c = i % CPR * E, row = r0 + r;
         const bool ok = r < rows && c < d.head_dim;
         cp_async16_or_zero(qs + r * P + c, (const T*)d.q + (ok ? (first + row / G) * d.q_stride + (kh * G + row % G) * d.q_head_stride + c : 0), ok);
@@ -90,7 +94,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_mma_kernel(const __grid_c
     int vis[2], row[2];
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-        row[e] = r0 + warp * 16 + g + 8 * e;
+        row[e] = r0 + wm * 16 + g + 8 * e;
         vis[e] = row[e] < n * G ? min(visible(p, len, n, row[e] / G), k_stop) : 0;
     }
     float o[NB][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
@@ -109,7 +113,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_mma_kernel(const __grid_c
             cp_async_commit();
         }
         const T* ks = kv + stage * 2 * BK * P;
-        const T* qw = qs + warp * 16 * P;
+        const T* qw = qs + wm * 16 * P;
         stage = stage + 1 == ST ? 0 : stage + 1;
         if constexpr (QREG) {
             if (t0 == k_beg)
@@ -117,8 +121,8 @@ __global__ void __launch_bounds__(kPagedThreads) paged_mma_kernel(const __grid_c
                 for (int k = 0; k < HD / 16; k++) ldsm4(qf[k], smem_u32(qw + (lane & 15) * P + k * 16 + (lane >> 4) * 8));
         }
 
-        const PaddedRows<T, P> kr{smem_u32(ks)}, vr{smem_u32(ks + BK * P)};
-        attend_keys<T, HD, BK / 8>(p, qw, qf, kr, vr, t0 + 2 * t, vis, m, l, o);
+        const PaddedRows<T, P> kr{smem_u32(ks + wk * KW * P)}, vr{smem_u32(ks + (BK + wk * KW) * P)};
+        attend_keys<T, HD, KW / 8>(p, qw, qf, kr, vr, t0 + wk * KW + 2 * t, vis, m, l, o);
     }
     cp_async_wait<0>();
 #pragma unroll
@@ -127,6 +131,36 @@ __global__ void __launch_bounds__(kPagedThreads) paged_mma_kernel(const __grid_c
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
     }
 
+    // join the two halves of the keys
+    __shared__ float2 half_ml[S::TR];
+    float* half_o = reinterpret_cast<float*>(kv);
+    __syncthreads();  // every stage is read
+    if (wk == 1)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int r = wm * 16 + g + 8 * e;
+            if (t == 0) half_ml[r] = make_float2(m[e], l[e]);
+#pragma unroll
+            for (int j = 0; j < NB; j++)
+                *reinterpret_cast<float2*>(half_o + r * S::MP + j * 8 + 2 * t) = make_float2(o[j][2 * e], o[j][2 * e + 1]);
+        }
+    __syncthreads();
+    if (wk == 1) return;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const int r = wm * 16 + g + 8 * e;
+        const float2 other = half_ml[r];
+        const float mm = fmaxf(m[e], other.x);
+        const float f0 = m[e] == -INFINITY ? 0.0f : ex2(m[e] - mm), f1 = other.x == -INFINITY ? 0.0f : ex2(other.x - mm);
+        m[e] = mm;
+        l[e] = l[e] * f0 + other.y * f1;
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            const float2 x = *reinterpret_cast<const float2*>(half_o + r * S::MP + j * 8 + 2 * t);
+            o[j][2 * e] = o[j][2 * e] * f0 + x.x * f1;
+            o[j][2 * e + 1] = o[j][2 * e + 1] * f0 + x.y * f1;
+        }
+    }
     // A row's result goes to out, or, when its keys fill more than one split, to this split's record.
 #pragma unroll
     for (int e = 0; e < 2; e++) {
@@ -271,7 +305,7 @@ static VoxCPMError paged_mma_launch(const PagedArgs& a, cudaStream_t st) {
     std::call_once(once, [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes); });
     VOXQ_CUDA_TRY(attr);
     const dim3 grid((int)((int64_t)a.d.total_q * a.group / S::TR) + a.d.batch, a.d.kv_heads, a.splits);
-    VOXQ_CUDA_TRY(launch_pdl(kern, grid, dim3(kPagedThreads), S::bytes, st, a));
+    VOXQ_CUDA_TRY(launch_pdl(kern, grid, dim3(kMmaThreads), S::bytes, st, a));
     return VOXCPM_SUCCESS;
 }
 

@@ -1,5 +1,6 @@
 #!/usr/bin/env python3
-"""Builds libvoxq.so (all CUDA sources for sm_100a) next to this file.
+"""Builds libvoxq.so (all CUDA sources for sm_100a) next to this file, and the binding of the batched
+operators to torch tensors (csrc/voxq_torch.cpp) as voxq/_torch.so.
 
     python voxcpm2-c_b200/build.py [-j N] [--force]
 
@@ -67,7 +68,30 @@ def build(force: bool = False, jobs: int = 8, verbose: bool = False) -> str:
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
+    build_binding(force)
     return LIB
+
+
+def build_binding(force: bool = False) -> str:
+    """voxq/_torch.so: a CPython module against the installed torch's headers and libraries."""
+    import sysconfig
+    import torch
+    src, out = os.path.join(CSRC, "voxq_torch.cpp"), os.path.join(HERE, "voxq", "_torch.so")
+    header = os.path.join(REPO, "include", "voxq.h")
+    if not force and os.path.exists(out) and os.path.getmtime(out) > max(os.path.getmtime(src), os.path.getmtime(header)):
+        return out
+    root = os.path.dirname(torch.__file__)
+    lib, inc = os.path.join(root, "lib"), os.path.join(root, "include")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w", src, "-o", out,
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(REPO, "include"),
+           "-I", cuda, "-I", sysconfig.get_paths()["include"], "-I", inc, "-I", os.path.join(inc, "torch", "csrc", "api", "include"),
+           "-L", lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", f"-Wl,-rpath,{lib}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError(f"g++ failed on {src}")
+    return out
 
 
 if __name__ == "__main__":

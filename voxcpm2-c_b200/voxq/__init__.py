@@ -13,7 +13,6 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -142,16 +141,6 @@ class LocEncDesc(C.Structure):
                 ("output_norm", C.POINTER(RmsNormDesc)), ("d_model", C.c_int), ("patch_size", C.c_int)]
 
 
-_PACK = {"p": "P", "l": "q", "i": "i", "f": "f", "d": "d", "z": "N"}
-
-
-def _packer(spec: str) -> "struct.Struct":
-    """The same fields as one struct.Struct in the C layout: packing a descriptor of some thirty fields takes a
-    quarter of the time of filling a ctypes Structure, which is most of a small call."""
-    return struct.Struct("".join(_PACK[part.split(":")[0].strip()] * len(part.split(":")[1].split())
-                                 for part in spec.split(";")) + "0P")
-
-
 def _fields(spec: str):
     """ctypes fields from "type: names" lines (p pointer, l int64, i int32, f float, d double, z size_t)."""
     types = {"p": C.c_void_p, "l": C.c_int64, "i": C.c_int32, "f": C.c_float, "d": C.c_double, "z": C.c_size_t}
@@ -166,38 +155,30 @@ class RopeTableDesc(C.Structure):
 
 class RopeDesc(C.Structure):
     """voxq_rope (include/voxq.h)."""
-    SPEC = ("p: q k v; l: q_stride q_head_stride k_stride k_head_stride v_stride v_head_stride; p: q_out; "
-            "l: qo_stride qo_head_stride; p: cache_k cache_v; l: page_stride row_stride head_stride; "
-            "p: freqs positions slots; i: tokens heads kv_heads head_dim rot_dim interleaved n_pos pages "
-            "page_size in_dtype cache_dtype")
-    _fields_ = _fields(SPEC)
-    pack = _packer(SPEC).pack
+    _fields_ = _fields("p: q k v; l: q_stride q_head_stride k_stride k_head_stride v_stride v_head_stride; p: q_out; "
+                       "l: qo_stride qo_head_stride; p: cache_k cache_v; l: page_stride row_stride head_stride; "
+                       "p: freqs positions slots; i: tokens heads kv_heads head_dim rot_dim interleaved n_pos pages "
+                       "page_size in_dtype cache_dtype")
 
 
 class PagedAttnDesc(C.Structure):
     """voxq_paged_attn (include/voxq.h)."""
-    SPEC = ("p: q; l: q_stride q_head_stride; p: out; l: o_stride o_head_stride; p: k v; "
-            "l: page_stride row_stride head_stride; p: block_table; l: table_stride; p: cu_q kv_len; "
-            "i: batch heads kv_heads head_dim pages page_size total_q max_q max_kv dtype out_dtype causal; "
-            "f: scale; p: workspace; z: workspace_bytes")
-    _fields_ = _fields(SPEC)
-    pack = _packer(SPEC).pack
+    _fields_ = _fields("p: q; l: q_stride q_head_stride; p: out; l: o_stride o_head_stride; p: k v; "
+                       "l: page_stride row_stride head_stride; p: block_table; l: table_stride; p: cu_q kv_len; "
+                       "i: batch heads kv_heads head_dim pages page_size total_q max_q max_kv dtype out_dtype causal; "
+                       "f: scale; p: workspace; z: workspace_bytes")
 
 
 class LoraDesc(C.Structure):
     """voxq_lora (include/voxq.h)."""
-    SPEC = ("p: x; l: ldx; p: base; l: ldb; p: out; l: ldo; p: a b cu adapter ranks scale; "
-            "i: rows batch K N rank adapters dtype w_dtype")
-    _fields_ = _fields(SPEC)
-    pack = _packer(SPEC).pack
+    _fields_ = _fields("p: x; l: ldx; p: base; l: ldb; p: out; l: ldo; p: a b cu adapter ranks scale; "
+                       "i: rows batch K N rank adapters dtype w_dtype")
 
 
 class NormDesc(C.Structure):
     """voxq_norm (include/voxq.h)."""
-    SPEC = ("p: y x gate; l: ldy ldx ldg; p: w_post w_pre gate_index h_out n_out; l: ldh ldn; "
-            "i: rows D gate_rows dtype; f: alpha eps")
-    _fields_ = _fields(SPEC)
-    pack = _packer(SPEC).pack
+    _fields_ = _fields("p: y x gate; l: ldy ldx ldg; p: w_post w_pre gate_index h_out n_out; l: ldh ldn; "
+                       "i: rows D gate_rows dtype; f: alpha eps")
 
 
 _vp, _sz, _i, _i64 = C.c_void_p, C.c_size_t, C.c_int, C.c_int64

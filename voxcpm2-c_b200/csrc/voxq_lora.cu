@@ -317,7 +317,8 @@ static VoxCPMError lora_launch(const voxq_lora& d, cudaStream_t st) {
         attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, LoraShape<T, W, TM>(RB * 8).bytes);
     });
     VOXQ_CUDA_TRY(attr);
-    // as many CTAs to a tile as it takes to fill the GPU twice, up to 8
+    // As many CTAs to a tile as keep the grid within 4 an SM, up to 8.  bf16 prompts (8000 rows, K 1024, N 4096, rank 32): 71 us
+    // with a bound of 2 an SM, 47 with 4, 50 with 8; 40 single rows: 12.8, 9.8 and 10.
     const int tiles = d.rows / TM + d.batch;
     int cl = 8;
     while (cl > 1 && (int64_t)tiles * cl > 4 * device_sm_count()) cl /= 2;
@@ -338,13 +339,18 @@ static VoxCPMError lora_launch(const voxq_lora& d, cudaStream_t st) {
     return VOXCPM_SUCCESS;
 }
 
-// Tiles of 64 rows read the weights less often, tiles of 16 waste fewer rows
-// on requests of a few.
+// Tiles of 64 rows read the weights less often and pay where there are enough of them and few are part empty; fp32 rows split
+// their operands for every MMA and want the more warps a row unless the rank is high.  us, 64 against 16 rows, bf16, rank 32,
+// K 1024, N 4096: 40 requests of 64 rows 35 : 31, of 128 49 : 51, of 300 80 : 104; 2 of 4096 47 : 55; rank 64, N 1024: 9 of
+// 1000 37 : 53.  fp32, rank 16, K = N = 2048: 9 of 1000 84 : 68, 2 of 4096 92 : 68; rank 64, K 1024, N 2048: 9 of 1000 123 : 150,
+// 40 of 300 227 : 219.
 template <typename T, typename W>
 static VoxCPMError lora_dispatch(const voxq_lora& d, cudaStream_t st) {
-    const bool tall = d.rows >= 24 * (int64_t)d.batch;
-    if (d.rank <= 32) return tall ? lora_launch<T, W, 64, 4>(d, st) : lora_launch<T, W, 16, 4>(d, st);
-    return tall ? lora_launch<T, W, 64, 16>(d, st) : lora_launch<T, W, 16, 16>(d, st);
+    const bool tall = d.rows >= 24 * (int64_t)d.batch && d.rows >= 32 * device_sm_count();
+    if (d.rank > 32) return tall ? lora_launch<T, W, 64, 16>(d, st) : lora_launch<T, W, 16, 16>(d, st);
+    if constexpr (!is_f32<T>)
+        if (tall) return lora_launch<T, W, 64, 4>(d, st);
+    return lora_launch<T, W, 16, 4>(d, st);
 }
 
 }  // namespace voxq

@@ -9,10 +9,13 @@
 
 namespace voxq {
 
-constexpr int kSplitCtas = 4;   // CTAs per SM that splitting the keys aims at
-constexpr int kTcSplitCtas = 1;  // the same for the tcgen05 kernel, one CTA of which fills an SM
-constexpr int kTcMinRows = 64;   // rows a sequence from which that kernel's 128-row tiles pay
-constexpr int kMinSplit = 256;  // keys that are worth a CTA of their own
+// Splits of the keys.  Down to kMinSplit keys while there is less than a CTA an SM: 8 fp32 tokens on 2000 keys took 31 us with
+// splits of 256, 16 with 64.  Down to kMinSplitMore while there are fewer than kSplitCtas an SM: 16 sequences of 32 fp32 tokens
+// on 1000 keys took 150 us with 2 an SM, 98 with 4, 96 with 8; finer, the records cost more than they save (12 tokens on 8000
+// keys, bf16 x 128: 22.5 us with 32 splits, 39 with 126).  The tcgen05 kernel, one CTA of which fills an SM, lasts as long for
+// 64 keys as for 200: 4 prompts of 200 tokens took 39 us split, 21 whole.
+constexpr int kMinSplit = 64, kMinSplitMore = 256, kSplitCtas = 4;
+constexpr int kTcWork = 48 * 1024;  // keys x head dims of 64-row tiles per SM from which the tcgen05 kernel pays
 constexpr int kMaxSplits = 128;
 
 constexpr int kMmaThreads = 256;
@@ -278,15 +281,20 @@ static PagedPlan paged_plan(const voxq_paged_attn& d) {
         r.bytes = paged_step_bytes(d);
         return r;
     }
-    r.tc = (int64_t)d.max_q * G > kTcMinRows && paged_tc_takes(d);
-    const int tr = r.tc ? kTcRows : 64, ctas = r.tc ? kTcSplitCtas : kSplitCtas;
-    // CTAs without splitting (at most one more than full tiles for every sequence), and the splits that bring them to
-    // `ctas` an SM without a second round
-    const int64_t tiles = ((int64_t)d.total_q * G / tr + std::min(d.batch, d.total_q)) * d.kv_heads;
-    const int64_t want = std::max<int64_t>(1, ctas * device_sm_count() / tiles);
-    const int64_t most = std::max<int64_t>(1, (d.max_kv + kMinSplit - 1) / kMinSplit);
-    const int64_t z = std::min(std::min(want, most), (int64_t)kMaxSplits);
-    r.split_len = (int)(((d.max_kv + z - 1) / z + 127) / 128 * 128);  // whole tiles of either kernel
+    // CTAs without splitting: at most one more than full tiles for every sequence
+    auto tiles_of = [&](int tr) { return ((int64_t)d.total_q * G / tr + std::min(d.batch, d.total_q)) * d.kv_heads; };
+    // The tcgen05 kernel starts up more slowly and is faster by key, so it takes the calls with much to do; sooner where
+    // there is more than a tile an SM, which the other kernel takes in turns.  us, this kernel against the MMAs, kv heads
+    // of 8 query heads x 128: a prompt of 50 tokens 16.4 : 12.3, of 400 31 : 27, 4 prompts of 200 20 : 27; 16 sequences of
+    // 3 tokens on 1500 keys 29 : 35, 64 of them 45 : 80.  x 64: 16 of 8 tokens 29 : 25, of 12 31 : 33, 64 of 12 37 : 59.
+    const int64_t small = tiles_of(64);
+    r.tc = paged_tc_takes(d) && (double)small * d.max_kv * d.head_dim >= (double)kTcWork * device_sm_count() / (small > device_sm_count() ? 2 : 1);
+    const int64_t tiles = tiles_of(r.tc ? kTcRows : 64), sms = device_sm_count();
+    auto splits = [&](int ctas, int keys) { return std::min(ctas * sms / tiles, ((int64_t)d.max_kv + keys - 1) / keys); };
+    const int64_t most = r.tc ? splits(1, kMinSplitMore) : std::max(splits(1, kMinSplit), splits(kSplitCtas, kMinSplitMore));
+    const int64_t z = std::min(std::max<int64_t>(1, most), (int64_t)kMaxSplits);
+    const int step = r.tc ? 128 : 64;  // whole key tiles
+    r.split_len = (int)(((d.max_kv + z - 1) / z + step - 1) / step * step);
     r.splits = r.split_len ? (d.max_kv + r.split_len - 1) / r.split_len : 1;
     if (r.splits <= 1) {
         r.splits = 1;
@@ -333,7 +341,7 @@ static VoxCPMError paged_check(const voxq_paged_attn* d) {
     if (d->max_kv && (d->page_size == 0 || d->pages == 0 || d->table_stride < (d->max_kv + (int64_t)d->page_size - 1) / d->page_size))
         return VOXCPM_ERR_SHAPE_MISMATCH;
     // row and tile numbers are 32-bit, and so are the launch grid's limits
-    if ((int64_t)d->total_q * d->heads + d->batch > INT32_MAX || d->heads > 65535 || d->max_kv > 1 << 30)
+    if ((int64_t)d->total_q * d->heads + (int64_t)d->batch * d->kv_heads > INT32_MAX || d->heads > 65535 || d->max_kv > 1 << 30)
         return VOXCPM_ERR_UNSUPPORTED;
     return VOXCPM_SUCCESS;
 }

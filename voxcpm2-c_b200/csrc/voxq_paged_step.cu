@@ -23,8 +23,11 @@ struct StepShape {
     static_assert(per_sm * (bytes + 2048) <= 228 * 1024, "shared memory");
 };
 constexpr int kStepThreads = 128;
-constexpr int kWholeTiles = 12;   // a row's keys stay in one block up to here
-constexpr int kMinTiles = 8;     // tiles that are worth a block of their own
+// A row's keys stay in one block up to kWholeTiles, or kWholeMany where the rows alone give half of the SMs a block: no join.
+// us, whole against cut, kv heads of 128: 1 sequence of 200 keys (7 tiles) 14 : 18, of 900 (29) 23 : 16; 64 of 700 25 : 29;
+// 128 of 1000 41 : 47.
+constexpr int kWholeTiles = 12, kWholeMany = 40;
+constexpr int kMinTiles = 4;  // tiles that are worth a block of their own: one sequence of 900 keys 16 us, 18 with 2 or 8, 25 with 16
 constexpr int kStepPieces = 512;  // most blocks, and so most pieces of one row
 
 // KT rows as 128-byte blocks of 128-byte-swizzled rows.
@@ -394,7 +397,7 @@ int paged_step_blocks(const voxq_paged_attn& d, int* whole) {
     const int64_t items = ((int64_t)d.total_q * group / 16 + std::min(d.batch, d.total_q)) * d.kv_heads;
     const int64_t tiles = std::max<int64_t>((d.max_kv + (int64_t)kt - 1) / kt, 1);
     const int64_t resident = std::min<int64_t>((d.head_dim > 128 ? 1 : 2) * device_sm_count(), kStepPieces);
-    *whole = tiles <= kWholeTiles;
+    *whole = tiles <= kWholeTiles || (tiles <= kWholeMany && items >= device_sm_count() / 2);
     return (int)std::max<int64_t>(1, std::min(resident, *whole ? items : items * tiles / kMinTiles));
 }
 

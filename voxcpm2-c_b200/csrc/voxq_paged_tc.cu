@@ -77,16 +77,6 @@ __device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t* v) {
                  VOXQ_S8(v, 0), VOXQ_S8(v, 8), VOXQ_S8(v, 16), VOXQ_S8(v, 24)
                  : "memory");
 }
-__device__ __forceinline__ void tm_ld16(uint32_t addr, uint32_t* v) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : VOXQ_R8(v, 0), VOXQ_R8(v, 8)
-                 : "r"(addr));
-}
-__device__ __forceinline__ void tm_st16(uint32_t addr, const uint32_t* v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
-                 VOXQ_S8(v, 0), VOXQ_S8(v, 8)
-                 : "memory");
-}
 __device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 

@@ -488,7 +488,10 @@ VOXQ_API VoxCPMError voxq_locenc_forward(const voxq_locenc_desc* enc, const Tens
  * cu[0] = 0 (device int32 [batch + 1]; a sequence may own none).
  *
  * All pointers are device pointers, all calls are asynchronous on `stream`,
- * allocate nothing and can be captured into a CUDA graph.  Element types are
+ * allocate nothing and can be captured into a CUDA graph -- but for the first
+ * voxq_paged_attention on a device, which makes the library's status word
+ * there (voxq_device_error: a bounded wait of its kernels that ran out; the
+ * call's results are then wrong), so let it not be a captured one.  Element types are
  * VOXQ_F32, VOXQ_F16 and VOXQ_BF16; sums, softmax statistics and norms are
  * fp32.  Strides are in elements; the last dimension is contiguous; base
  * addresses and strides must be multiples of 16 bytes where a comment says

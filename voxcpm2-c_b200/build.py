@@ -86,7 +86,7 @@ def build_binding(force: bool = False) -> str:
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-w", src, "-o", out,
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(REPO, "include"),
            "-I", cuda, "-I", sysconfig.get_paths()["include"], "-I", inc, "-I", os.path.join(inc, "torch", "csrc", "api", "include"),
-           "-L", lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", f"-Wl,-rpath,{lib}"]
+           "-L", lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", f"-Wl,-rpath,{lib}"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)

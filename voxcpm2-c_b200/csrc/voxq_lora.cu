@@ -11,13 +11,13 @@ constexpr int kLoraThreads = 128;
 constexpr int kLoraWarps = kLoraThreads / 32;
 constexpr int kLoraMaxRank = 128;
 
-// Shape of the kernel for x of type T, weights of type W and TM rows a tile.
-template <typename T, typename W, int TM>
+// Shape of the kernel for x of type T, weights of type W, TM rows a tile and NB output columns a step.
+template <typename T, typename W, int TM, int COLS>
 struct LoraShape {
     static constexpr int WM = TM / 16;                // warps along the rows
     static constexpr int WK = kLoraWarps / WM;        // warps along K (first product) or the columns (second)
     static constexpr int KB = is_f32<W> || TM == 64 ? 64 : 128;  // K per stage: four blocks of TM 64 share an SM
-    static constexpr int NB = TM == 64 ? 64 : 128;    // output columns per step
+    static constexpr int NB = COLS;
     static constexpr int NW = NB / WK;                // of a warp
     static constexpr int XP = KB + 16 / sizeof(T);    // shared pitches: 16 bytes more than a row, so that the 8 rows
     static constexpr int AP = KB + 16 / sizeof(W);    // of a fragment load lie in different banks
@@ -90,7 +90,8 @@ __device__ __forceinline__ void mul_16(float (*d)[4], const T* as, const T* as_l
 // NB columns of B[w] from n0 on, [column][rank], to shared memory; zeros past N and past the adapter's own rank r (what
 // lies there may be anything).  Within a warp's NW columns, column c goes to row (c % CW / 2) * 8 + 2 (c / CW) + c % 2
 // with CW = NW / 4: the columns that a thread gets from the MMAs -- 2 t and 2 t + 1 of every block of 8 rows -- are then
-// CW neighbours of the output, and base and out move straight between memory and the accumulators.  per: 16-byte vectors of a column, inv: 2^20 / per rounded up.
+// CW neighbours of the output, and base and out move straight between memory and the accumulators.  per: 16-byte vectors
+// of a column, inv: 2^20 / per rounded up.
 template <typename W, int NB, int NW>
 __device__ __forceinline__ void load_b(W* dst, int bp, const W* b, int n0, int N, int rank, int r, int per, uint32_t inv) {
     constexpr int E = 16 / sizeof(W);
@@ -127,9 +128,13 @@ __device__ __forceinline__ void load_b(W* dst, int bp, const W* b, int n0, int N
 // enters the second product unrounded to 16 significant bits or more (two
 // 16-bit parts, or TF32 parts), because a 16-bit h would cost as much accuracy
 // as the output's own rounding.
-template <typename T, typename W, int TM, int RB>
+// 40 single fp32 rows, K = N = 2048, rank 16: 8.2 us (19 with a block a row and no cluster).  9 bf16 prompts, 8000 rows, K
+// 1024, N 4096, ranks up to 32: 48 us, 2.4 TB/s, against 17 at HBM's rate: 17 000 clocks to h, then 3500 a column
+// step of a block (wait for B, the products, base, store), which four blocks an SM overlap only in part; a deeper
+// prefetch of B or base gained nothing.
+template <typename T, typename W, int TM, int RB, int COLS>
 __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constant__ voxq_lora d) {
-    using S = LoraShape<T, W, TM>;
+    using S = LoraShape<T, W, TM, COLS>;
     constexpr int WM = S::WM, WK = S::WK, KB = S::KB, NB = S::NB, NW = S::NW;
     extern __shared__ __align__(16) uint8_t lora_sh[];
     const S z(d.rank);
@@ -307,14 +312,15 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
     if (r > 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <typename T, typename W, int TM, int RB>
+template <typename T, typename W, int TM, int RB, int COLS>
 static VoxCPMError lora_launch(const voxq_lora& d, cudaStream_t st) {
-    const LoraShape<T, W, TM> z(d.rank);
+    using S = LoraShape<T, W, TM, COLS>;
+    const S z(d.rank);
     static std::once_flag once;
     static cudaError_t attr = cudaSuccess;
-    auto kern = lora_kernel<T, W, TM, RB>;
+    auto kern = lora_kernel<T, W, TM, RB, COLS>;
     std::call_once(once, [&] {
-        attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, LoraShape<T, W, TM>(RB * 8).bytes);
+        attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S(RB * 8).bytes);
     });
     VOXQ_CUDA_TRY(attr);
     // As many CTAs to a tile as keep the grid within 4 an SM, up to 8.  bf16 prompts (8000 rows, K 1024, N 4096, rank 32): 71 us
@@ -343,14 +349,15 @@ static VoxCPMError lora_launch(const voxq_lora& d, cudaStream_t st) {
 // their operands for every MMA and want the more warps a row unless the rank is high.  us, 64 against 16 rows, bf16, rank 32,
 // K 1024, N 4096: 40 requests of 64 rows 35 : 31, of 128 49 : 51, of 300 80 : 104; 2 of 4096 47 : 55; rank 64, N 1024: 9 of
 // 1000 37 : 53.  fp32, rank 16, K = N = 2048: 9 of 1000 84 : 68, 2 of 4096 92 : 68; rank 64, K 1024, N 2048: 9 of 1000 123 : 150,
-// 40 of 300 227 : 219.
+// 40 of 300 227 : 219.  Steps of 256 columns where they keep the eight CTAs of a cluster busy, of 128 else: 40 single rows,
+// N 2048, 8.3 : 9.8; N 1024, 18 : 16.
 template <typename T, typename W>
 static VoxCPMError lora_dispatch(const voxq_lora& d, cudaStream_t st) {
     const bool tall = d.rows >= 24 * (int64_t)d.batch && d.rows >= 32 * device_sm_count();
-    if (d.rank > 32) return tall ? lora_launch<T, W, 64, 16>(d, st) : lora_launch<T, W, 16, 16>(d, st);
+    if (d.rank > 32) return tall ? lora_launch<T, W, 64, 16, 64>(d, st) : lora_launch<T, W, 16, 16, 128>(d, st);
     if constexpr (!is_f32<T>)
-        if (tall) return lora_launch<T, W, 64, 4>(d, st);
-    return lora_launch<T, W, 16, 4>(d, st);
+        if (tall) return lora_launch<T, W, 64, 4, 64>(d, st);
+    return d.N >= 2048 ? lora_launch<T, W, 16, 4, 256>(d, st) : lora_launch<T, W, 16, 4, 128>(d, st);
 }
 
 }  // namespace voxq

@@ -73,8 +73,9 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 // rows, by the latency of one load and two reductions for a few.  WR warps
 // hold a whole row in registers, PER vectors of V elements a thread, so the
 // second norm needs no second read; all of a row's loads are issued before the
-// first reduction.
-// h stays fp32 from its sum to the norm.
+// first reduction.  h stays fp32 from its sum to the norm.  8191 bf16 rows of
+// 1024, gated, with both norms: 18.4 us, 3.6 TB/s with inputs partly in L2; 2
+// fp32 rows of 2048: 2.3 us.
 template <typename T, int V, int WR, int PER>
 __global__ void __launch_bounds__(WR == 1 ? 128 : 32 * WR) norm_residual_kernel(const __grid_constant__ voxq_norm d) {
     __shared__ float red[2][WR];

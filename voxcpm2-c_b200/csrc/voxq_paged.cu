@@ -15,7 +15,7 @@ namespace voxq {
 // keys, bf16 x 128: 22.5 us with 32 splits, 39 with 126).  The tcgen05 kernel, one CTA of which fills an SM, lasts as long for
 // 64 keys as for 200: 4 prompts of 200 tokens took 39 us split, 21 whole.
 constexpr int kMinSplit = 64, kMinSplitMore = 256, kSplitCtas = 4;
-constexpr int kTcWork = 48 * 1024;  // keys x head dims of 64-row tiles per SM from which the tcgen05 kernel pays
+constexpr int kTcWork = 36 * 1024;  // keys x head dims of 64-row tiles per SM from which the tcgen05 kernel pays
 constexpr int kMaxSplits = 128;
 
 constexpr int kMmaThreads = 256;
@@ -43,6 +43,9 @@ struct PagedShape {
 // anywhere inside it); rows past the end are zeros in shared memory, whatever the cache holds.  One pass, base-2 softmax
 // with running maximum m and sum l per row.  With few tiles the keys are split over CTAs (blockIdx.z); a row with more
 // than one split leaves (m, l, sums) for paged_combine_kernel.
+// 5 sequences of 21..133 fp32 tokens on 300..1500 keys, 16 query heads over 2 x 64: 46 us, 20 TFLOP/s of fp32-accurate
+// products (58 with one warp a row group and all of a tile's keys).  Bound by the latency of its MMAs and, in fp32, by
+// splitting every operand into two TF32 parts on its way to them: 8 instructions for three MMAs' worth of work.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kMmaThreads) paged_mma_kernel(const __grid_constant__ PagedArgs p) {
     using S = PagedShape<T, HD>;
@@ -190,7 +193,7 @@ __global__ void __launch_bounds__(kMmaThreads) paged_mma_kernel(const __grid_con
 
 // Joins a row's splits in their order: M = max m_z, out = sum_z acc_z 2^(m_z - M) / sum_z l_z 2^(m_z - M).  One CTA per
 // token and head, its warps along the splits: with a thread per element that walked all of them, 50 splits took longer
-// than the attention itself.
+// than the attention itself.  Latency bound: 4 us behind the attention, most of it the start and two dependent loads.
 template <typename T>
 __global__ void __launch_bounds__(kPagedThreads) paged_combine_kernel(const __grid_constant__ PagedArgs p) {
     constexpr int W = kPagedThreads / 32;
@@ -281,15 +284,13 @@ static PagedPlan paged_plan(const voxq_paged_attn& d) {
         r.bytes = paged_step_bytes(d);
         return r;
     }
-    // CTAs without splitting: at most one more than full tiles for every sequence
-    auto tiles_of = [&](int tr) { return ((int64_t)d.total_q * G / tr + std::min(d.batch, d.total_q)) * d.kv_heads; };
-    // The tcgen05 kernel starts up more slowly and is faster by key, so it takes the calls with much to do; sooner where
-    // there is more than a tile an SM, which the other kernel takes in turns.  us, this kernel against the MMAs, kv heads
-    // of 8 query heads x 128: a prompt of 50 tokens 16.4 : 12.3, of 400 31 : 27, 4 prompts of 200 20 : 27; 16 sequences of
-    // 3 tokens on 1500 keys 29 : 35, 64 of them 45 : 80.  x 64: 16 of 8 tokens 29 : 25, of 12 31 : 33, 64 of 12 37 : 59.
-    const int64_t small = tiles_of(64);
-    r.tc = paged_tc_takes(d) && (double)small * d.max_kv * d.head_dim >= (double)kTcWork * device_sm_count() / (small > device_sm_count() ? 2 : 1);
-    const int64_t tiles = tiles_of(r.tc ? kTcRows : 64), sms = device_sm_count();
+    // The tcgen05 kernel starts up more slowly and is faster by key, so it takes the calls with much to do; sooner where the
+    // tiles alone come near one an SM.  us, this kernel against the MMAs, kv heads of 8 query heads x 128: a prompt of 50
+    // tokens 16 : 12, of 400 33 : 29, 4 prompts of 200 20 : 29; 16 sequences of 3 tokens on 1500 keys 31 : 35, 64 of them
+    // 45 : 80, 64 of 4 on 300 22 : 35.  x 64: 16 of 8 on 1500 29 : 25, of 12 31 : 33, 64 of 12 37 : 59.
+    const int64_t small = paged_tiles(d, 64), sms = device_sm_count();
+    r.tc = paged_tc_takes(d) && (double)small * d.max_kv * d.head_dim >= (double)kTcWork * sms / (4 * small > 3 * sms ? 3 : 1);
+    const int64_t tiles = paged_tiles(d, r.tc ? kTcRows : 64);
     auto splits = [&](int ctas, int keys) { return std::min(ctas * sms / tiles, ((int64_t)d.max_kv + keys - 1) / keys); };
     const int64_t most = r.tc ? splits(1, kMinSplitMore) : std::max(splits(1, kMinSplit), splits(kSplitCtas, kMinSplitMore));
     const int64_t z = std::min(std::max<int64_t>(1, most), (int64_t)kMaxSplits);

@@ -233,6 +233,15 @@ __device__ __forceinline__ void tma_page(uint32_t dst, const PagedMaps& m, const
                  : "memory");
 }
 
+// Tiles of tr rows, pairs (token, head of the group), that a call can have for all its kv heads: at most one more than full
+// tiles for every sequence, and as many a sequence as the longest has.
+inline int64_t paged_tiles(const voxq_paged_attn& d, int tr) {
+    const int64_t group = d.heads / d.kv_heads, every = d.total_q * group / tr + (d.batch < d.total_q ? d.batch : d.total_q),
+                  longest = d.max_q < d.total_q ? d.max_q : d.total_q, most = (longest * group + tr - 1) / tr * d.batch;
+    const int64_t tiles = every < most ? every : most;
+    return (tiles > 1 ? tiles : 1) * d.kv_heads;
+}
+
 constexpr int kPagedThreads = 128;
 constexpr int kPagedMaxHeadDim = 256;
 // At most 16 rows a sequence (voxq_paged_step.cu), caches that paged_maps_take: everything that the call needs, and the

@@ -72,8 +72,10 @@ __device__ __forceinline__ int step_blocks(const PagedArgs& p, int64_t total) {
 // joined.  It also issues its own TMA copies, a lane per box of a page, SW tiles ahead and on into the next row's keys;
 // boxes past the last key are left out, and the pages of the tile after next are looked up meanwhile.  (One warp that
 // issues for all took 700 clocks a tile, most of them for the copies' operands, and was the bound of short calls; the
-// same stages by cp.async took 65 to 150 us where this takes 38 for 64 sequences of 600..4096 keys, 3.9 TB/s, since a warp has few of those in
-// flight.)  Two blocks share an SM: one's start and joins hide behind the other's stream.
+// same stages by cp.async took 65 to 150 us where this takes 38 for 64 sequences of 600..4096 keys x 2 heads x 128, 3.9 TB/s,
+// since a warp has few of those in flight.)  Two blocks share an SM: one's start and joins hide behind the other's
+// stream (with 4 or 6, of smaller stages, 46 and 54 us).  Of the 38 us 1.5 pass before the first tile, blocks end
+// between 24 and 32, and the join takes the rest.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kStepThreads, StepShape<T, HD>::per_sm) paged_step_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ PagedMaps maps) {
     using S = StepShape<T, HD>;

@@ -175,6 +175,12 @@ __device__ __forceinline__ bool next_block(const uint4* answer, int& x, int& y, 
 // A block stays for many units (the grid is one block per unit; the running ones take over the rest): the loader and
 // the first scores of a unit run ahead of the previous one's output, and tensor memory, barriers and shared memory are
 // set up once.  Every wait is bounded and records the device error word.
+// 6 causal prompts of 1500..4096 tokens, 16 query heads over 2 kv heads x 128, bf16 (279 GFLOP): 285 us in a short burst,
+// 0.98 PFLOP/s; 315 us over and over, when the power limit lowers the clocks.  (One block a unit, in the order of the batch,
+// with a maximum before the weights: 380 us.)  Bound by the chain of a key tile: the softmax warps wait 1300 clocks for the
+// scores, read them in 70, take 1450 for maximum, exponentials (at 16 a clock an SM alone 1024 for both tiles) and
+// rounding, 220 to write the weights; a unit's output and next queries add 8500.  One or two tiles that fill the machine
+// once (3 sequences of 40..64 tokens on 12 000 keys: 37 us) pay that start and end and the join for one short run.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ PagedMaps maps) {
     constexpr int TILE = kTcTileBytes<HD>, ST = kTcStages;
@@ -759,7 +765,9 @@ static VoxCPMError tc_launch(const PagedArgs& a, cudaStream_t st) {
     PagedMaps m;
     const VoxCPMError e = paged_maps(d, kTcTile, &m);
     if (e != VOXCPM_SUCCESS) return e;
-    const dim3 grid(((int)((int64_t)d.total_q * a.group / kTcRows) + d.batch) * d.kv_heads, 1, a.splits);
+    // a block for every unit there can be (the search of many sequences numbers one more a sequence)
+    const dim3 grid(d.batch <= 32 * kTcSeqs ? (int)paged_tiles(d, kTcRows) : ((int)((int64_t)d.total_q * a.group / kTcRows) + d.batch) * d.kv_heads, 1,
+                    a.splits);
     VOXQ_CUDA_TRY(launch_pdl(kern, grid, dim3(kTcThreads), kTcSmem<HD>, st, a, m));
     return VOXCPM_SUCCESS;
 }

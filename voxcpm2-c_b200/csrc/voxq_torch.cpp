@@ -8,8 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <ATen/ops/empty.h>
-#include <ATen/ops/empty_like.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -89,6 +88,11 @@ int i32(int64_t v) {
 }
 void* stream_of(const at::Tensor& like) { return (void*)c10::cuda::getCurrentCUDAStream(like.get_device()).stream(); }
 
+// Memory of the current stream, contiguous, without the dispatcher's half microsecond a tensor.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& beside) {
+    return at::detail::empty_cuda(sizes, type, beside.device(), std::nullopt);
+}
+
 template <typename F>
 PyObject* guarded(Py_ssize_t have, Py_ssize_t want, F f) {
     if (have != want) {
@@ -122,7 +126,7 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
              "q [T, heads, D] and k, v [T, kv_heads, D] of one type are needed");
         caches(ck, cv, D);
         need(ck.size(2) == KVH, "the caches' kv_heads differ from k's");
-        at::Tensor out = given ? *given : at::empty_like(q, q.options().dtype(ck.scalar_type()));
+        at::Tensor out = given ? *given : fresh(q.sizes(), ck.scalar_type(), q);
         need(rows_ok(out, 3) && out.sizes() == q.sizes() && out.scalar_type() == ck.scalar_type(), "q_out: q's shape and the caches' type, on the GPU");
         voxq_rope d{};
         if (freqs) {
@@ -179,7 +183,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         d.max_q = as_i32(a[6], "max_q is past 2^31");
         d.max_kv = as_i32(a[7], "max_kv is past 2^31");
         need(d.max_kv <= bt.size(1) * ck.size(1), "max_kv is more than the block table's pages hold");
-        at::Tensor out = given ? *given : at::empty_like(q);
+        at::Tensor out = given ? *given : fresh(q.sizes(), q.scalar_type(), q);
         need(rows_ok(out, 3) && out.sizes() == q.sizes(), "out: q's shape, contiguous along head_dim, on the GPU");
         d.q = q.const_data_ptr();
         d.q_stride = q.stride(0);
@@ -210,7 +214,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const size_t bytes = g.paged_workspace(&d);
         at::Tensor ws;
         if (bytes) {
-            ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+            ws = fresh({(int64_t)bytes}, at::kByte, q);
             d.workspace = ws.data_ptr();
             d.workspace_bytes = bytes;
         }
@@ -232,7 +236,7 @@ PyObject* lora(PyObject*, PyObject* const* o, Py_ssize_t n) {
         const int64_t M = x.size(0), N = b.size(1), B = who.numel(), nA = a.size(0);
         auto fits = [&](const at::Tensor& t) { return rows_ok(t, 2) && t.size(0) == M && t.size(1) == N && t.scalar_type() == x.scalar_type(); };
         need(!base || fits(*base), "base: [rows, N] of x's type, contiguous along N, on the GPU");
-        at::Tensor out = given ? *given : base ? at::empty_like(*base) : at::empty({M, N}, x.options());
+        at::Tensor out = given ? *given : fresh({M, N}, x.scalar_type(), x);
         need(fits(out), "out: [rows, N] of x's type, contiguous along N, on the GPU");
         voxq_lora d{};
         d.x = x.const_data_ptr();
@@ -285,10 +289,10 @@ PyObject* norm_residual(PyObject*, PyObject* const* a, Py_ssize_t n) {
         }
         if (w_post) d.w_post = (const float*)vec(*w_post, D, at::kFloat, "w_post: a contiguous CUDA vector of D fp32");
         if (w_pre) d.w_pre = (const float*)vec(*w_pre, D, at::kFloat, "w_pre: a contiguous CUDA vector of D fp32");
-        at::Tensor h = h_given ? *h_given : at::empty_like(y), nn;
+        at::Tensor h = h_given ? *h_given : fresh(y.sizes(), y.scalar_type(), y), nn;
         need(fits(h), "h_out: [rows, D] of y's type, contiguous along D, on the GPU");
         if (w_pre) {
-            nn = n_given ? *n_given : at::empty_like(y);
+            nn = n_given ? *n_given : fresh(y.sizes(), y.scalar_type(), y);
             need(fits(nn), "n_out: [rows, D] of y's type, contiguous along D, on the GPU");
             d.n_out = nn.data_ptr();
             d.ldn = nn.stride(0);

@@ -181,6 +181,15 @@ def test_paged_attention_many_units(causal, dim, dtype):
     attend(n, [a + rng.randint(0, 300) for a in n], 16, 2, dim, 16, dtype, causal, seed=dim)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+@pytest.mark.parametrize("dim", [8, 40, 80, 120, 136, 200, 256])
+@pytest.mark.parametrize("n,lens", [([700, 90, 0, 33], [1500, 90, 7, 900]), ([5] * 70, [800 + 3 * i for i in range(70)])])
+def test_paged_attention_head_dims_on_many_rows(n, lens, dim, dtype):
+    """Head dims below the kernels' own, in calls with enough to do for the tensor-memory kernel."""
+    attend(n, lens, 18, 3, dim, 16, dtype, seed=dim)
+    attend(n, lens, 18, 3, dim, 16, dtype, False, seed=dim, out_dtype=F32)
+
+
 @pytest.mark.parametrize("n,lens", [([1] * 5, [3000, 20, 400, 1, 800]), ([190, 40], [300, 2500])])
 def test_paged_attention_same_bits_and_other_streams(n, lens):
     """The same bits on every run, on a side stream and inside a CUDA graph."""
@@ -357,6 +366,14 @@ def test_lora(rows, nA, K, N, r, dt, wt):
         R.assert_within(voxq.lora(x, a, b, cu, who, scale, base=bs, ranks=rk), ref, bound, f"ranks {rk is not None}")
 
 
+@pytest.mark.parametrize("dt,wt", [(F32, F32), (F16, F16)], ids=ids)
+@pytest.mark.parametrize("r", [24, 40, 64, 72])
+@pytest.mark.parametrize("rows", [[1] * 50, [900, 0, 2100, 37, 1900]])
+def test_lora_ranks_and_row_counts(rows, r, dt, wt):
+    """Every rank class with tiles of 16 and of 64 rows."""
+    test_lora(rows, 5, 328, 2184, r, dt, wt)
+
+
 @pytest.mark.parametrize("dt,wt", [(F32, BF16), (BF16, BF16)], ids=ids)
 @pytest.mark.parametrize("rows", [[1, 1, 1], [100, 3, 40]])
 def test_lora_in_place_strided_and_unused(rows, dt, wt):
@@ -400,6 +417,20 @@ def test_norm_residual(M, D, post, gate, pre, dtype):
         R.assert_within(n, *nn, "n")
     else:
         assert n is None
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("D", [250, 258, 514, 1002, 2047, 2050, 4095, 4102, 8190, 9001])
+def test_norm_residual_narrow_widths(D, dtype):
+    """Widths that only two elements, or one, an access divide."""
+    g = torch.Generator(device="cuda").manual_seed(D)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    y, x, gt = rnd(37, D).to(dtype), rnd(37, D).to(dtype), rnd(1, D).to(dtype)
+    w_pre, w_post = 1 + 0.1 * rnd(D), 1 + 0.1 * rnd(D)
+    h, n = voxq.norm_residual(y, x, w_pre, w_post, gt, alpha=0.7, eps=1e-6)
+    (hr, hb), nn = R.norm_residual(y, x, w_pre, w_post, gt, None, 0.7, 1e-6)
+    R.assert_within(h, hr, hb, "h")
+    R.assert_within(n, *nn, "n")
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)

@@ -1,4 +1,5 @@
 // voxq_lora.cu -- low-rank adapters of many requests beside a shared projection.
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -129,7 +130,7 @@ __device__ __forceinline__ void load_b(W* dst, int bp, const W* b, int n0, int N
 // 16-bit parts, or TF32 parts), because a 16-bit h would cost as much accuracy
 // as the output's own rounding.
 // 40 single fp32 rows, K = N = 2048, rank 16: 8.2 us (19 with a block a row and no cluster).  9 bf16 prompts, 8000 rows, K
-// 1024, N 4096, ranks up to 32: 48 us, 2.4 TB/s, against 17 at HBM's rate: 17 000 clocks to h, then 3500 a column
+// 1024, N 4096, ranks up to 32: 42 us, 2.7 TB/s, against 17 at HBM's rate: 17 000 clocks to h, then 3500 a column
 // step of a block (wait for B, the products, base, store), which four blocks an SM overlap only in part; a deeper
 // prefetch of B or base gained nothing.
 template <typename T, typename W, int TM, int RB, int COLS>
@@ -323,11 +324,13 @@ static VoxCPMError lora_launch(const voxq_lora& d, cudaStream_t st) {
         attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S(RB * 8).bytes);
     });
     VOXQ_CUDA_TRY(attr);
-    // As many CTAs to a tile as keep the grid within 4 an SM, up to 8.  bf16 prompts (8000 rows, K 1024, N 4096, rank 32): 71 us
-    // with a bound of 2 an SM, 47 with 4, 50 with 8; 40 single rows: 12.8, 9.8 and 10.
+    // As many CTAs to a tile as keep the grid within 4 an SM, up to 8.  Where 4 fit an SM any number, else a power of two, which
+    // leaves no holes in a second round.  bf16 prompts (8000 rows, K 1024, N 4096, rank 32): 42 us, 47 with powers of two, 71
+    // with a bound of 2 an SM and 50 with 8; 9 of 1000 rows, rank 64, K 2960, N 1032: 59 us, 78 with any number.
     const int tiles = d.rows / TM + d.batch;
-    int cl = 8;
-    while (cl > 1 && (int64_t)tiles * cl > 4 * device_sm_count()) cl /= 2;
+    int cl = std::min(8, std::max(1, 4 * device_sm_count() / tiles));
+    if (z.bytes + 1024 > 227 * 1024 / 4)
+        while (cl & (cl - 1)) cl--;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles * cl);
     cfg.blockDim = dim3(kLoraThreads);
@@ -349,12 +352,13 @@ static VoxCPMError lora_launch(const voxq_lora& d, cudaStream_t st) {
 // their operands for every MMA and want the more warps a row unless the rank is high.  us, 64 against 16 rows, bf16, rank 32,
 // K 1024, N 4096: 40 requests of 64 rows 35 : 31, of 128 49 : 51, of 300 80 : 104; 2 of 4096 47 : 55; rank 64, N 1024: 9 of
 // 1000 37 : 53.  fp32, rank 16, K = N = 2048: 9 of 1000 84 : 68, 2 of 4096 92 : 68; rank 64, K 1024, N 2048: 9 of 1000 123 : 150,
-// 40 of 300 227 : 219.  Steps of 256 columns where they keep the eight CTAs of a cluster busy, of 128 else: 40 single rows,
+// 40 of 300 227 : 219; bf16, rank 64, K 2960, N 1032: 30 of 96 37 : 51, 40 of 64 37 : 33, 4 of 40 22 : 16.  Steps of 256 columns where they keep the eight CTAs of a cluster busy, of 128 else: 40 single rows,
 // N 2048, 8.3 : 9.8; N 1024, 18 : 16.
 template <typename T, typename W>
 static VoxCPMError lora_dispatch(const voxq_lora& d, cudaStream_t st) {
-    const bool tall = d.rows >= 24 * (int64_t)d.batch && d.rows >= 32 * device_sm_count();
-    if (d.rank > 32) return tall ? lora_launch<T, W, 64, 16, 64>(d, st) : lora_launch<T, W, 16, 16, 128>(d, st);
+    const bool tall = d.rows >= 24 * (int64_t)d.batch && d.rows >= (d.rank > 32 && !is_f32<T> ? 16 : 32) * device_sm_count();
+    if (d.rank > 64) return tall ? lora_launch<T, W, 64, 16, 64>(d, st) : lora_launch<T, W, 16, 16, 128>(d, st);
+    if (d.rank > 32) return tall ? lora_launch<T, W, 64, 8, 64>(d, st) : lora_launch<T, W, 16, 8, 128>(d, st);
     if constexpr (!is_f32<T>)
         if (tall) return lora_launch<T, W, 64, 4, 64>(d, st);
     return d.N >= 2048 ? lora_launch<T, W, 16, 4, 256>(d, st) : lora_launch<T, W, 16, 4, 128>(d, st);

@@ -7,8 +7,12 @@ namespace voxq {
 
 constexpr int kNormMaxD = 16384;
 
-// V contiguous elements in one access (16 bytes, or one element where a row
-// or its width is not 16-byte aligned).
+// V contiguous elements in one access: 16 bytes, or two elements or one where a
+// row or its width is not aligned to more.
+template <int BYTES>
+struct VecAccess {
+    using type = typename std::conditional<BYTES == 16, uint4, typename std::conditional<BYTES == 8, uint2, typename std::conditional<BYTES == 4, uint32_t, uint16_t>::type>::type>::type;
+};
 template <typename T, int V>
 struct Vec {
     T e[V];
@@ -16,23 +20,17 @@ struct Vec {
 template <typename T, int V>
 __device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
     Vec<T, V> r;
-    if constexpr (V > 1) {
-        const uint4 v = *reinterpret_cast<const uint4*>(p);
-        memcpy(&r, &v, 16);
-    } else {
-        r.e[0] = *p;
-    }
+    using A = typename VecAccess<V * sizeof(T)>::type;
+    const A v = *reinterpret_cast<const A*>(p);
+    memcpy(&r, &v, sizeof(A));
     return r;
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& r) {
-    if constexpr (V > 1) {
-        uint4 v;
-        memcpy(&v, &r, 16);
-        *reinterpret_cast<uint4*>(p) = v;
-    } else {
-        *p = r.e[0];
-    }
+    using A = typename VecAccess<V * sizeof(T)>::type;
+    A v;
+    memcpy(&v, &r, sizeof(A));
+    *reinterpret_cast<A*>(p) = v;
 }
 
 // The norm weights go through the read-only path, so that their loads may be
@@ -41,6 +39,10 @@ template <int V>
 __device__ __forceinline__ void load_weights(float (&w)[V], const float* p) {
     if constexpr (V == 1) {
         w[0] = __ldg(p);
+    } else if constexpr (V == 2) {
+        const float2 v = __ldg(reinterpret_cast<const float2*>(p));
+        w[0] = v.x;
+        w[1] = v.y;
     } else {
 #pragma unroll
         for (int i = 0; i < V / 4; i++) {
@@ -158,14 +160,26 @@ static cudaError_t norm_launch(const voxq_norm& d, cudaStream_t st) {
     return launch_pdl(norm_residual_kernel<T, V, WR, PER>, dim3(blocks), dim3(WR == 1 ? 128 : 32 * WR), 0, st, d);
 }
 
+// Widths and alignments that are not 16-byte: two elements or one an access, so several a thread, and room for no more than
+// the row needs.  (3289 gated rows of 2162 in fp16, both norms: 32 us; 160 with one element an access and room for 16 384.)
+template <typename T, int V>
+static cudaError_t norm_narrow(const voxq_norm& d, cudaStream_t st) {
+    const int nv = (d.D + V - 1) / V;
+    if (nv <= 256) return norm_launch<T, V, 4, 2>(d, st);
+    if (nv <= 512) return norm_launch<T, V, 4, 4>(d, st);
+    if (nv <= 1024) return norm_launch<T, V, 8, 4>(d, st);
+    if (nv <= 2048) return norm_launch<T, V, 16, 4>(d, st);
+    if (nv <= 4096) return norm_launch<T, V, 16, 8>(d, st);
+    return norm_launch<T, V, 16, kNormMaxD / 512 / V>(d, st);
+}
+
 // One vector a thread as far as 512 threads go: the shortest chains and the most rows in flight.  (8191 rows of 1024 in
 // bf16, gated, with both norms: 24.6 us from cold caches with 4 warps of one vector a row, 26.6 with one warp of four,
 // 28.7 with 4 warps and room for two.)
 template <typename T>
-static cudaError_t norm_dispatch(const voxq_norm& d, bool wide, cudaStream_t st) {
+static cudaError_t norm_dispatch(const voxq_norm& d, int width, cudaStream_t st) {
     constexpr int V = 16 / sizeof(T);
-    if (!wide)  // odd widths and alignments, one element per access
-        return d.D <= 1024 ? norm_launch<T, 1, 4, 8>(d, st) : norm_launch<T, 1, 16, 32>(d, st);
+    if (width < V) return width == 2 ? norm_narrow<T, 2>(d, st) : norm_narrow<T, 1>(d, st);
     const int nv = d.D / V;
     if (nv <= 32) return norm_launch<T, V, 1, 1>(d, st);
     if (nv <= 64) return norm_launch<T, V, 2, 1>(d, st);
@@ -189,9 +203,15 @@ extern "C" VoxCPMError voxq_norm_residual(const voxq_norm* d, void* stream) {
     if (d->gate && (d->gate_rows == 0 || (!d->gate_index && d->gate_rows != 1 && d->gate_rows != d->rows)))
         return VOXCPM_ERR_SHAPE_MISMATCH;
     const int dt = d->dtype;
-    const bool wide = d->D % (16 / elem_bytes(dt)) == 0 && rows16(d->y, d->ldy, dt) && rows16(d->x, d->ldx, dt) &&
-                      (!d->gate || rows16(d->gate, d->ldg, dt)) && (!d->h_out || rows16(d->h_out, d->ldh, dt)) &&
-                      (!d->n_out || rows16(d->n_out, d->ldn, dt)) && rows16(d->w_post, 0, VOXQ_F32) && rows16(d->w_pre, 0, VOXQ_F32);
-    VOXQ_CUDA_TRY(with_elem(dt, [&](auto x) { return norm_dispatch<decltype(x)>(*d, wide, (cudaStream_t)stream); }));
+    // elements per access: the most that divide the width and to which all rows are aligned
+    auto fits = [&](int v) {
+        const int64_t by = (int64_t)v * elem_bytes(dt);
+        auto rows = [&](const void* p, int64_t ld) { return !p || ((uintptr_t)p % by == 0 && ld * elem_bytes(dt) % by == 0); };
+        auto weights = [&](const float* w) { return (uintptr_t)w % (v < 4 ? 4 * v : 16) == 0; };
+        return d->D % v == 0 && rows(d->y, d->ldy) && rows(d->x, d->ldx) && rows(d->gate, d->ldg) && rows(d->h_out, d->ldh) &&
+               rows(d->n_out, d->ldn) && weights(d->w_post) && weights(d->w_pre);
+    };
+    const int wide = 16 / elem_bytes(dt), width = fits(wide) ? wide : fits(2) ? 2 : 1;
+    VOXQ_CUDA_TRY(with_elem(dt, [&](auto x) { return norm_dispatch<decltype(x)>(*d, width, (cudaStream_t)stream); }));
     return VOXCPM_SUCCESS;
 }

@@ -33,8 +33,8 @@ struct PagedShape {
     static_assert(bytes <= 227 * 1024 && TR * MP * 4 <= ST * stage, "shared memory");
 };
 
-// Attention of more than 16 rows a sequence on warp-level MMAs: fp32, and the head dims and page sizes that the tcgen05
-// kernel does not take; and any number of rows where a tensor map cannot describe the caches.
+// Attention of more than 16 rows a sequence on warp-level MMAs: fp32, calls with little to do, and the head dims and page
+// sizes that the tcgen05 kernel does not take; and any number of rows where a tensor map cannot describe the caches.
 //
 // The rows of a tile are the pairs (token, query head of the kv head's group), so a key is read once for all heads that
 // share it.  Two warps own each 16 rows and take half of a tile's keys each, with their own maximum and sums, joined at the

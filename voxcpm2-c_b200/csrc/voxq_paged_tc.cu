@@ -172,6 +172,7 @@ __device__ __forceinline__ bool next_block(const uint4* answer, int& x, int& y, 
 // knows that every earlier PV is complete too: it may rescale O without a barrier of its own.  Rescaling is rare: sums
 // stay relative to a maximum that may be up to 2^8 behind (exact: p, l and O share it).  p is rounded to the operand
 // type, l sums the fp32 values.
+// Head dims below HD are zeros in shared memory: the tensor maps end there, and the queries are written so.
 // A block stays for many units (the grid is one block per unit; the running ones take over the rest): the loader and
 // the first scores of a unit run ahead of the previous one's output, and tensor memory, barriers and shared memory are
 // set up once.  Every wait is bounded and records the device error word.
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
             for (int i = 0; i < CPR; i++) {
                 v[i] = make_uint4(0, 0, 0, 0);
-                if (row0 + i * STEP < u.rows)
+                if (row0 + i * STEP < u.rows && cj * 8 < d.head_dim)
                     v[i] = *reinterpret_cast<const uint4*>((const T*)d.q + (u.first + tok) * d.q_stride + (u.kh * G + h) * d.q_head_stride + cj * 8);
                 for (h += STEP; h >= G; h -= G) tok++;
             }
@@ -633,7 +634,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 const int r = next.r0 + t * kTcTile + lr;
                 const T* src = (const T*)d.q + (next.first + r / G) * d.q_stride + (next.kh * G + r % G) * d.q_head_stride;
 #pragma unroll
-                for (int c = 0; c < HD; c += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + c));
+                for (int c = 0; c < HD; c += 64)
+                    if (c < d.head_dim) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + c));
             }
             if (ok && tiles > 0) {
                 ok = warp_wait(o_done + t, unit++ & 1, VOXQ_DEVERR_WAIT_MMA, p.err);
@@ -648,7 +650,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 const float inv = !whole ? 1.0f : seen > 0 ? 1.0f / l : 0.0f;
                 const int64_t rec = ((int64_t)(it.first + tok) * d.heads + h) * p.splits + it.z;
                 if (put && !whole) p.ml[rec] = make_float2(m, l);
-                const int64_t dst = whole ? (it.first + tok) * d.o_stride + h * d.o_head_stride : rec * HD;
+                const int64_t dst = whole ? (it.first + tok) * d.o_stride + h * d.o_head_stride : rec * d.head_dim;
                 const int kind = !put ? 0 : whole ? 1 : 2;
                 // 16-bit rows of the output at once, fp32 ones (records, or an fp32 output) in two halves of the head
                 const bool fast = d.out_dtype != VOXQ_F32 && __all_sync(0xffffffffu, kind < 2);
@@ -679,7 +681,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                         const int row = crow + i * STEP, what = __shfl_sync(0xffffffffu, kind, row);
                         const int64_t at = __shfl_sync(0xffffffffu, dst, row);
                         const uint4 v = lds128(place(row, cj));
-                        if (what == 0) continue;
+                        if (what == 0 || part * (HD / 2) + cj * (fast ? 8 : 4) >= d.head_dim) continue;
                         if (fast) {
                             *reinterpret_cast<uint4*>((T*)d.out + at + cj * 8) = v;
                         } else {
@@ -751,7 +753,7 @@ VoxCPMError paged_maps(const voxq_paged_attn& d, int max_rows, PagedMaps* m) {
 }
 
 bool paged_tc_takes(const voxq_paged_attn& d) {
-    return d.dtype != VOXQ_F32 && (d.head_dim == 64 || d.head_dim == 128) && d.scale >= 0.0f && paged_maps_take(d);
+    return d.dtype != VOXQ_F32 && d.head_dim <= 128 && d.scale >= 0.0f && paged_maps_take(d);
 }
 
 template <typename T, int HD>
@@ -773,8 +775,8 @@ static VoxCPMError tc_launch(const PagedArgs& a, cudaStream_t st) {
 }
 
 VoxCPMError paged_tc_launch(const PagedArgs& a, cudaStream_t st) {
-    if (a.d.dtype == VOXQ_F16) return a.d.head_dim == 64 ? tc_launch<__half, 64>(a, st) : tc_launch<__half, 128>(a, st);
-    return a.d.head_dim == 64 ? tc_launch<bf16, 64>(a, st) : tc_launch<bf16, 128>(a, st);
+    if (a.d.dtype == VOXQ_F16) return a.d.head_dim <= 64 ? tc_launch<__half, 64>(a, st) : tc_launch<__half, 128>(a, st);
+    return a.d.head_dim <= 64 ? tc_launch<bf16, 64>(a, st) : tc_launch<bf16, 128>(a, st);
 }
 
 }  // namespace voxq

@@ -290,7 +290,7 @@ static PagedPlan paged_plan(const voxq_paged_attn& d) {
     // 45 : 80, 64 of 4 on 300 22 : 35.  x 64: 16 of 8 on 1500 29 : 25, of 12 31 : 33, 64 of 12 37 : 59.
     const int64_t small = paged_tiles(d, 64), sms = device_sm_count();
     r.tc = paged_tc_takes(d) && (double)small * d.max_kv * d.head_dim >= (double)kTcWork * sms / (4 * small > 3 * sms ? 3 : 1);
-    const int64_t tiles = paged_tiles(d, r.tc ? kTcRows : 64);
+    const int64_t tiles = paged_tiles(d, r.tc ? paged_tc_rows(d) : 64);
     auto splits = [&](int ctas, int keys) { return std::min(ctas * sms / tiles, ((int64_t)d.max_kv + keys - 1) / keys); };
     const int64_t most = r.tc ? splits(1, kMinSplitMore) : std::max(splits(1, kMinSplit), splits(kSplitCtas, kMinSplitMore));
     const int64_t z = std::min(std::max<int64_t>(1, most), (int64_t)kMaxSplits);

@@ -248,9 +248,9 @@ constexpr int kPagedMaxHeadDim = 256;
 // workspace that it takes.  VOXCPM_ERR_UNSUPPORTED, like paged_tc_launch, for a layout that a tensor map cannot describe.
 size_t paged_step_bytes(const voxq_paged_attn& d);
 VoxCPMError paged_step_launch(const PagedArgs& a, cudaStream_t st);
-// Attention on the tcgen05 tensor cores (voxq_paged_tc.cu): 16-bit types, head_dim up to 128, scale >= 0, caches that
+// Attention on the tcgen05 tensor cores (voxq_paged_tc.cu): 16-bit types, scale >= 0, caches that
 // paged_maps_take.  Launches the main kernel only.
-constexpr int kTcRows = 256;  // rows of a CTA
+int paged_tc_rows(const voxq_paged_attn& d);  // rows of a CTA
 bool paged_tc_takes(const voxq_paged_attn& d);
 VoxCPMError paged_tc_launch(const PagedArgs& a, cudaStream_t st);
 

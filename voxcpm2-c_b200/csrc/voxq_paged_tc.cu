@@ -11,7 +11,10 @@ namespace voxq {
 constexpr int kTcTile = 128;                 // rows of a query tile, keys of a key tile
 constexpr int kTcThreads = 384;              // two softmax warpgroups; loader, MMA and unit warps, one idle
 constexpr int kTcRegsSoftmax = 208, kTcRegsOther = 80;  // 256 * 208 + 128 * 80 <= the 384 * 168 of the launch
-constexpr int kTcStages = 5;                 // ring of key and value tiles
+template <int HD>
+constexpr int kTcTiles = HD > 128 ? 1 : 2;   // query tiles of a unit: tensor memory holds the output of 256 columns once
+template <int HD>
+constexpr int kTcStages = HD > 128 ? 2 : 5;  // ring of key and value tiles
 constexpr int kTcHalf = kTcTile * 128;       // bytes of 128 rows x 64 dims, 128-byte-swizzled rows
 constexpr int kTcItems = 4;                  // units in flight between the warps of a block
 constexpr int kTcSeqs = 4;                   // of 32 sequences: up to how many the units are taken in order of their keys
@@ -20,7 +23,7 @@ constexpr float kTcSlack = 8.0f;             // how far a row's maximum may grow
 template <int HD>
 constexpr int kTcTileBytes = kTcHalf * (HD / 64);
 template <int HD>
-constexpr int kTcSmem = (2 + kTcStages) * kTcTileBytes<HD> + 1024;
+constexpr int kTcSmem = (kTcTiles<HD> + kTcStages<HD>) * kTcTileBytes<HD> + 1024;
 
 // Operand descriptors, 128-byte swizzle, 8-row groups 1024 bytes apart.
 // K-major (queries, keys): a row holds 64 of the inner dimension.
@@ -172,7 +175,9 @@ __device__ __forceinline__ bool next_block(const uint4* answer, int& x, int& y, 
 // knows that every earlier PV is complete too: it may rescale O without a barrier of its own.  Rescaling is rare: sums
 // stay relative to a maximum that may be up to 2^8 behind (exact: p, l and O share it).  p is rounded to the operand
 // type, l sums the fp32 values.
-// Head dims below HD are zeros in shared memory: the tensor maps end there, and the queries are written so.
+// Head dims below HD are zeros in shared memory: the tensor maps end there, and the queries are written so.  HD 256: one
+// query tile a unit and a ring of two, so that a tile's softmax waits for its products and they for it; 4 prompts of 300
+// tokens on 1000 keys 111 us, 0.2 PFLOP/s, where the MMA kernel takes 252.
 // A block stays for many units (the grid is one block per unit; the running ones take over the rest): the loader and
 // the first scores of a unit run ahead of the previous one's output, and tensor memory, barriers and shared memory are
 // set up once.  Every wait is bounded and records the device error word.
@@ -184,7 +189,7 @@ __device__ __forceinline__ bool next_block(const uint4* answer, int& x, int& y, 
 // once (3 sequences of 40..64 tokens on 12 000 keys: 37 us) pay that start and end and the join for one short run.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ PagedMaps maps) {
-    constexpr int TILE = kTcTileBytes<HD>, ST = kTcStages;
+    constexpr int TILE = kTcTileBytes<HD>, ST = kTcStages<HD>, TW = kTcTiles<HD>, ROWS = TW * kTcTile;
     extern __shared__ uint8_t tc_raw[];
     __shared__ uint64_t bar[2 * ST + 2 * kTcItems + 12];
     __shared__ uint4 answer;
@@ -196,7 +201,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     uint64_t *item_full = q_full + 2, *item_empty = item_full + kTcItems, *tail = item_empty + kTcItems, *asked = tail + 2, *begun = asked + 1;
     const voxq_paged_attn& d = p.d;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, G = p.group;
-    const uint32_t qsm = (smem_u32(tc_raw) + 1023) & ~1023u, ring = qsm + 2 * TILE;
+    const uint32_t qsm = (smem_u32(tc_raw) + 1023) & ~1023u, ring = qsm + TW * TILE;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < ST; i++) {
@@ -333,7 +338,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                     uint32_t sk = slot;
                     advance();
 #pragma unroll
-                    for (int t = 0; t < 2; t++) {
+                    for (int t = 0; t < TW; t++) {
                         if (t && !two) break;
                         ok = ok && mbar_wait_bounded(q_full + t, units[t]++ & 1, VOXQ_DEVERR_WAIT_FULL, p.err, kTcLong);
                         tc_after();
@@ -362,7 +367,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                         const uint64_t vd = desc_mn(ring + sv * TILE);
                         const uint32_t now_v = sv, now_k = sk;
 #pragma unroll
-                        for (int t = 0; t < 2; t++) {
+                        for (int t = 0; t < TW; t++) {
                             if (t && !two) break;
                             ok = ok && mbar_wait_bounded(p_full + t, steps_done[t]++ & 1, VOXQ_DEVERR_WAIT_MMA, p.err);
                             tc_after();
@@ -376,11 +381,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                                 if (t == (two ? 1 : 0)) tc_commit(empty + now_v);
                                 tc_commit(o_done + t);
                             }
-                            if (t == 0 && more) fetch(i + 2 < tiles);  // the next step's tiles, while tile 1's softmax works
+                            if (TW > 1 && t == 0 && more) fetch(i + 2 < tiles);  // the next step's tiles, while tile 1's softmax works
                         }
                         if (!ok || !more) break;
                         tc_commit(empty + now_v);
                         tc_commit(empty + now_k);
+                        if (TW == 1) fetch(i + 2 < tiles);  // (into the slots that are being freed)
                     }
                 }
                 ok = __all_sync(0xffffffffu, ok);
@@ -406,7 +412,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 const int i = j * 32 + lane;
                 const bool in = sorted && i < d.batch;
                 const int first = in ? __ldg(d.cu_q + i) : 0, n = in ? min(__ldg(d.cu_q + i + 1), d.total_q) - first : 0;
-                seq_units[j] = first >= 0 && n > 0 ? (n * G + kTcRows - 1) / kTcRows : 0;
+                seq_units[j] = first >= 0 && n > 0 ? (n * G + ROWS - 1) / ROWS : 0;
                 seq_len[j] = in ? min(max(__ldg(d.kv_len + i), 0), d.max_kv) : 0;
                 seq_past[j] = seq_len[j] - n;
             }
@@ -415,8 +421,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 if (v < 0) return seq_units[j];
                 if (seq_len[j] <= v || seq_units[j] == 0) return 0;
                 if (!d.causal) return seq_units[j];
-                // all but the last unit end on a multiple of kTcRows rows: unit r is past v from (v - past) * G / kTcRows on
-                return 1 + min(max(seq_units[j] - 1 - (int)((int64_t)max(v - seq_past[j], 0) * G / kTcRows), 0), max(seq_units[j] - 1, 0));
+                // all but the last unit end on a multiple of ROWS rows: unit r is past v from (v - past) * G / ROWS on
+                return 1 + min(max(seq_units[j] - 1 - (int)((int64_t)max(v - seq_past[j], 0) * G / ROWS), 0), max(seq_units[j] - 1, 0));
             };
             auto above = [&](int v) {
                 int c = 0;
@@ -460,16 +466,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                     const int tile = gridDim.x / d.kv_heads - 1 - nth;
                     for (int i0 = 0; i0 < d.batch; i0 += 32) {
                         const int i = i0 + lane;
-                        s += __popc(__ballot_sync(0xffffffffu, i < d.batch && __ldg(d.cu_q + i) * G / kTcRows + i <= tile));
+                        s += __popc(__ballot_sync(0xffffffffu, i < d.batch && __ldg(d.cu_q + i) * G / ROWS + i <= tile));
                     }
                     s = max(s, 0);
-                    r = tile - (__ldg(d.cu_q + s) * G / kTcRows + s);
+                    r = tile - (__ldg(d.cu_q + s) * G / ROWS + s);
                 }
                 it.table = max(s, 0);
                 it.first = __ldg(d.cu_q + it.table);
                 it.n = s < 0 ? 0 : min(__ldg(d.cu_q + s + 1), d.total_q) - it.first;
-                it.r0 = r * kTcRows;
-                it.rows = min(it.n * G - it.r0, kTcRows);
+                it.r0 = r * ROWS;
+                it.rows = min(it.n * G - it.r0, ROWS);
                 it.len = min(max(__ldg(d.kv_len + it.table), 0), d.max_kv);
                 it.kh = kh;
                 it.z = z;
@@ -512,16 +518,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         auto load_q = [&](const TcItem& u) {
             const int row0 = t * kTcTile + (warp & 3) * 32 + crow, r = u.r0 + row0;
             int tok = r / G, h = r % G;
-            uint4 v[CPR];
+            constexpr int BATCH = CPR < 16 ? CPR : 16;
+            uint4 v[BATCH];
 #pragma unroll
-            for (int i = 0; i < CPR; i++) {
-                v[i] = make_uint4(0, 0, 0, 0);
-                if (row0 + i * STEP < u.rows && cj * 8 < d.head_dim)
-                    v[i] = *reinterpret_cast<const uint4*>((const T*)d.q + (u.first + tok) * d.q_stride + (u.kh * G + h) * d.q_head_stride + cj * 8);
-                for (h += STEP; h >= G; h -= G) tok++;
+            for (int i0 = 0; i0 < CPR; i0 += BATCH) {
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) {
+                    v[i] = make_uint4(0, 0, 0, 0);
+                    if (row0 + (i0 + i) * STEP < u.rows && cj * 8 < d.head_dim)
+                        v[i] = *reinterpret_cast<const uint4*>((const T*)d.q + (u.first + tok) * d.q_stride + (u.kh * G + h) * d.q_head_stride + cj * 8);
+                    for (h += STEP; h >= G; h -= G) tok++;
+                }
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) sts128(place(crow + (i0 + i) * STEP, cj), v[i]);
             }
-#pragma unroll
-            for (int i = 0; i < CPR; i++) sts128(place(crow + i * STEP, cj), v[i]);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full + t);
@@ -752,8 +762,10 @@ VoxCPMError paged_maps(const voxq_paged_attn& d, int max_rows, PagedMaps* m) {
     return VOXCPM_SUCCESS;
 }
 
+int paged_tc_rows(const voxq_paged_attn& d) { return kTcTile * (d.head_dim > 128 ? kTcTiles<256> : kTcTiles<128>); }
+
 bool paged_tc_takes(const voxq_paged_attn& d) {
-    return d.dtype != VOXQ_F32 && d.head_dim <= 128 && d.scale >= 0.0f && paged_maps_take(d);
+    return d.dtype != VOXQ_F32 && d.scale >= 0.0f && paged_maps_take(d);
 }
 
 template <typename T, int HD>
@@ -768,15 +780,16 @@ static VoxCPMError tc_launch(const PagedArgs& a, cudaStream_t st) {
     const VoxCPMError e = paged_maps(d, kTcTile, &m);
     if (e != VOXCPM_SUCCESS) return e;
     // a block for every unit there can be (the search of many sequences numbers one more a sequence)
-    const dim3 grid(d.batch <= 32 * kTcSeqs ? (int)paged_tiles(d, kTcRows) : ((int)((int64_t)d.total_q * a.group / kTcRows) + d.batch) * d.kv_heads, 1,
-                    a.splits);
+    const int rows = paged_tc_rows(d);
+    const dim3 grid(d.batch <= 32 * kTcSeqs ? (int)paged_tiles(d, rows) : ((int)((int64_t)d.total_q * a.group / rows) + d.batch) * d.kv_heads, 1, a.splits);
     VOXQ_CUDA_TRY(launch_pdl(kern, grid, dim3(kTcThreads), kTcSmem<HD>, st, a, m));
     return VOXCPM_SUCCESS;
 }
 
 VoxCPMError paged_tc_launch(const PagedArgs& a, cudaStream_t st) {
-    if (a.d.dtype == VOXQ_F16) return a.d.head_dim <= 64 ? tc_launch<__half, 64>(a, st) : tc_launch<__half, 128>(a, st);
-    return a.d.head_dim <= 64 ? tc_launch<bf16, 64>(a, st) : tc_launch<bf16, 128>(a, st);
+    const int hd = a.d.head_dim;
+    if (a.d.dtype == VOXQ_F16) return hd <= 64 ? tc_launch<__half, 64>(a, st) : hd <= 128 ? tc_launch<__half, 128>(a, st) : tc_launch<__half, 256>(a, st);
+    return hd <= 64 ? tc_launch<bf16, 64>(a, st) : hd <= 128 ? tc_launch<bf16, 128>(a, st) : tc_launch<bf16, 256>(a, st);
 }
 
 }  // namespace voxq

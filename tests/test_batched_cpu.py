@@ -173,3 +173,19 @@ def test_paged_cache_places():
 def test_block_refuses_adapters_beside_the_fused_pair():
     with pytest.raises(ValueError):
         BatchedBlock(*[None] * 9, heads=1, kv_heads=1, adapters={"w1": None})
+
+
+def test_binding_refuses_host_tensors_and_other_objects():
+    z = torch.zeros
+    ints = z(2, dtype=torch.int32)
+    cache = z(2, 16, 2, 64)
+    for f, args in ((voxq.paged_attention, (z(1, 4, 64), cache, cache, z(1, 2, dtype=torch.int32), ints, ints[:1], 1, 16)),
+                    (voxq.rope_append, (z(1, 4, 64), z(1, 2, 64), z(1, 2, 64), None, None, z(1, dtype=torch.int64), cache, cache)),
+                    (voxq.lora, (z(2, 64), z(1, 8, 64), z(1, 32, 8), ints, ints[:1], z(1))),
+                    (voxq.norm_residual, (z(2, 64), z(2, 64)))):
+        with pytest.raises(ValueError):
+            f(*args)
+        with pytest.raises(ValueError):
+            f(None, *args[1:])
+        with pytest.raises(ValueError):
+            f([1.0], *args[1:])

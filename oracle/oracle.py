@@ -81,13 +81,14 @@ def dequantize(blocks, n: int, qtype: int, q8_signed: bool = False) -> np.ndarra
     return out
 
 
-def matmul_nt(a, w) -> np.ndarray:
+def matmul_nt(a, w, out=None) -> np.ndarray:
     """out = a @ w.T with one sequential fp32 accumulator (src/tensor.c:666-675)."""
     a, ap = _f32(a)
     w, wp = _f32(w)
     M, K = a.shape
     N = w.shape[0]
-    out = np.zeros((M, N), dtype=np.float32)
+    if out is None:
+        out = np.zeros((M, N), dtype=np.float32)
     lib().oracle_matmul_nt(ap, wp, out.ctypes.data_as(C.POINTER(C.c_float)), M, N, K)
     return out
 

@@ -495,3 +495,16 @@ def test_refusals():
     assert e.value.code == voxq.SHAPE_MISMATCH
     with pytest.raises(ValueError):
         voxq.norm_residual(x, x, one)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,lens", [([1, 1], [300, 700]), ([120, 40], [300, 700])])
+def test_paged_attention_fp32_is_as_close_as_fp32(n, lens, dim):
+    """The error over the whole output, as a norm: 2^-20 is sixteen roundings of fp32, where single TF32 products or long
+    sums inside the MMAs give more."""
+    pool = Pool(lens, 16, 2, dim, F32)
+    q = torch.randn(sum(n), 8, dim, device="cuda")
+    cu, kv = ints(starts(n)), ints(lens)
+    o = voxq.paged_attention(q, pool.k, pool.v, pool.table, cu, kv, max(n), max(lens))
+    ref, _ = R.attention(q, torch.nan_to_num(pool.k), torch.nan_to_num(pool.v), pool.table, cu, kv, True, dim ** -0.5, None)
+    assert float((R.f8(o) - ref).norm() / ref.norm()) < 2.0 ** -20

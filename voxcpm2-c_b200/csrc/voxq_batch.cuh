@@ -84,11 +84,12 @@ __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x as a sum of two TF32 values: what is left out is below 2^-22 of it.
+// x as a sum of two TF32 values, the high one rounded to nearest, the low one cut: what is left out is below 2^-22 of it.
+// In integer operations, as conversions run at a fraction of their rate (5 sequences of 80 fp32 tokens on 1200 keys: 80 us,
+// 94 with conversions).  A NaN whose bits the rounding carries over stays one in the low part.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    const float r = x - __uint_as_float(hi);
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(r));
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 
 // Calls f with a value of the element type that `dtype` names.

@@ -203,8 +203,20 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
             __syncthreads();
             const T* xs = reinterpret_cast<const T*>(lora_sh + (c & 1) * z.stage) + wm * 16 * S::XP;
             const W* as = reinterpret_cast<const W*>(reinterpret_cast<const T*>(lora_sh + (c & 1) * z.stage) + TM * S::XP);
-            for (int k = wk * 16; k < KB; k += WK * 16)
-                mul_16<T, W, RB, false>(acc, xs + k, nullptr, S::XP, as + k, S::AP, blocks);
+            if constexpr (is_f32<T>) {  // (MMA accumulation truncates: fp32 sums leave it after every stage)
+                float part[RB][4];
+#pragma unroll
+                for (int i = 0; i < RB; i++) part[i][0] = part[i][1] = part[i][2] = part[i][3] = 0.0f;
+                for (int k = wk * 16; k < KB; k += WK * 16)
+                    mul_16<T, W, RB, false>(part, xs + k, nullptr, S::XP, as + k, S::AP, blocks);
+#pragma unroll
+                for (int i = 0; i < RB; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][e] += part[i][e];
+            } else {
+                for (int k = wk * 16; k < KB; k += WK * 16)
+                    mul_16<T, W, RB, false>(acc, xs + k, nullptr, S::XP, as + k, S::AP, blocks);
+            }
             __syncthreads();
         }
         // this CTA's part of h: [K part of a warp][row][rank]

@@ -43,9 +43,9 @@ struct PagedShape {
 // anywhere inside it); rows past the end are zeros in shared memory, whatever the cache holds.  One pass, base-2 softmax
 // with running maximum m and sum l per row.  With few tiles the keys are split over CTAs (blockIdx.z); a row with more
 // than one split leaves (m, l, sums) for paged_combine_kernel.
-// 5 sequences of 21..133 fp32 tokens on 300..1500 keys, 16 query heads over 2 x 64: 46 us, 20 TFLOP/s of fp32-accurate
-// products (58 with one warp a row group and all of a tile's keys).  Bound by the latency of its MMAs and, in fp32, by
-// splitting every operand into two TF32 parts on its way to them: 8 instructions for three MMAs' worth of work.
+// 5 sequences of 21..133 fp32 tokens on 300..1500 keys, 16 query heads over 2 x 64: 40 us, 23 TFLOP/s of fp32-accurate
+// products (58 with one warp a row group, all of a tile's keys and conversions for the split).  Bound by the latency of its
+// MMAs and, in fp32, by splitting every operand into two TF32 parts on its way to them.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kMmaThreads) paged_mma_kernel(const __grid_constant__ PagedArgs p) {
     using S = PagedShape<T, HD>;

@@ -76,8 +76,9 @@ struct PaddedRows {
 
 // One step of a warp: its 16 rows against 8 KN keys.  16-bit types: m16n8k16 with fp32 accumulation; the weights p
 // enter the second product as two 16-bit parts, since one would cost as much accuracy as the output's own rounding.
-// fp32: three TF32 products per operand pair (high and low parts), the second product's sums started afresh each step
-// and added in fp32, because MMA accumulation truncates.  qs: the rows' queries in shared memory (16-bit types with
+// fp32: three TF32 products per operand pair (high and low parts).  MMA accumulation truncates, so no sum is left in it for
+// long: the scores' go over in fp32 every 64 dims, the low parts' stay apart, the second product's start afresh each step
+// (with one chain of three MMAs a step the error at 256 dims was 2e-6, three to seven times a plain fp32 product's).  qs: the rows' queries in shared memory (16-bit types with
 // HD <= 128 take them from the registers qf instead), pitch HD + 16 bytes; ks(row, dim), vs(row, dim): shared addresses
 // of the keys and values; base: the position
 // of this lane's first score column (2 t into the keys); vis: what rows g and g + 8 see; m, l, o: running maxima, this
@@ -109,23 +110,40 @@ __device__ __forceinline__ void attend_keys(const PagedArgs& p, const T* qs, con
             }
         }
     } else {
-#pragma unroll 4
-        for (int k = 0; k < HD; k += 8) {
-            uint32_t ah[4], al[4];
-            split_tf32(qs[g * P + k + t], ah[0], al[0]);
-            split_tf32(qs[(g + 8) * P + k + t], ah[1], al[1]);
-            split_tf32(qs[g * P + k + t + 4], ah[2], al[2]);
-            split_tf32(qs[(g + 8) * P + k + t + 4], ah[3], al[3]);
+        float low[KN][4];
 #pragma unroll
-            for (int j = 0; j < KN; j++) {
-                uint32_t bh[2], bl[2];
-                split_tf32(lds_f32(ks(j * 8 + g, k + t)), bh[0], bl[0]);
-                split_tf32(lds_f32(ks(j * 8 + g, k + t + 4)), bh[1], bl[1]);
-                mma8(sc[j], al, bh[0], bh[1]);
-                mma8(sc[j], ah, bl[0], bl[1]);
-                mma8(sc[j], ah, bh[0], bh[1]);
+        for (int j = 0; j < KN; j++) low[j][0] = low[j][1] = low[j][2] = low[j][3] = 0.0f;
+#pragma unroll 1
+        for (int k0 = 0; k0 < HD; k0 += 64) {
+            float a[KN][4];
+#pragma unroll
+            for (int j = 0; j < KN; j++) a[j][0] = a[j][1] = a[j][2] = a[j][3] = 0.0f;
+#pragma unroll 4
+            for (int k = k0; k < k0 + 64; k += 8) {
+                uint32_t ah[4], al[4];
+                split_tf32(qs[g * P + k + t], ah[0], al[0]);
+                split_tf32(qs[(g + 8) * P + k + t], ah[1], al[1]);
+                split_tf32(qs[g * P + k + t + 4], ah[2], al[2]);
+                split_tf32(qs[(g + 8) * P + k + t + 4], ah[3], al[3]);
+#pragma unroll
+                for (int j = 0; j < KN; j++) {
+                    uint32_t bh[2], bl[2];
+                    split_tf32(lds_f32(ks(j * 8 + g, k + t)), bh[0], bl[0]);
+                    split_tf32(lds_f32(ks(j * 8 + g, k + t + 4)), bh[1], bl[1]);
+                    mma8(low[j], al, bh[0], bh[1]);
+                    mma8(low[j], ah, bl[0], bl[1]);
+                    mma8(a[j], ah, bh[0], bh[1]);
+                }
             }
+#pragma unroll
+            for (int j = 0; j < KN; j++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) sc[j][c] += a[j][c];
         }
+#pragma unroll
+        for (int j = 0; j < KN; j++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) sc[j][c] += low[j][c];
     }
 
     // masks, the rows' maxima over the quad, weights

@@ -564,9 +564,12 @@ VOXQ_API VoxCPMError voxq_rope_append(const voxq_rope* d, void* stream);
  * a row that sees no key gives zeros.  Query head h reads kv head
  * h / (heads / kv_heads).  Position j of sequence s is row j % page_size of
  * page block_table[s][j / page_size] (entries outside [0, pages) read page
- * 0); page_size is any number.  Cache rows at or past kv_len may hold anything, NaN
- * included.  q, k, v are one type; out is that type or VOXQ_F32.  In the 16-bit types the products take
- * 16-bit operands with fp32 accumulation.  max_q and max_kv are upper bounds
+ * 0); page_size is any number.  Cache rows at or past kv_len may hold
+ * anything, NaN included.  q, k, v are one type; out is that type or VOXQ_F32.
+ * In the 16-bit types the products take 16-bit operands with fp32
+ * accumulation.  The softmax weights enter the second product with 16
+ * significant bits or more when out is VOXQ_F32, and otherwise with at least as
+ * many as out keeps (8 in bf16, 11 in fp16).  max_q and max_kv are upper bounds
  * of the sequences' new tokens and lengths (they choose the kernel and size
  * its grid; kv_len is clamped to max_kv).  16-byte rows; head_dim a multiple
  * of 8 up to 256; heads / kv_heads any whole number.

@@ -1,0 +1,32 @@
+"""The batched-step operators on the GPU where types, sizes and values meet their limits."""
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+import batched_ref as R  # noqa: E402
+import voxq  # noqa: E402
+from test_gpu_batched import BF16, F16, F32, Pool, ids, ints, starts  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+# ||out - ref|| / ||ref|| of an fp32 output over 16-bit operands.  The values have mean zero, so an error of relative size
+# e in every weight gives e in this norm: weights rounded once to the operand type give their rounding's root mean square,
+# 2^-8 / sqrt(12) .. 2^-7 / sqrt(12) in bf16 (over 2^-10) and 2^-13 or more in fp16; in two parts the square of that, under
+# 2^-16 and 2^-22.  The bounds are 2^4 under the one and over the other for bf16, and 2^3 or more for fp16, where fp32's
+# own errors (scores of 128 products: under 2^-20) are what is left.
+TWO_PARTS = {BF16: 2.0 ** -13, F16: 2.0 ** -17}
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,lens", [([1] * 4, [64, 208, 48, 160]), ([40, 24], [64, 48]), ([48] * 70, [48, 64] * 35),
+                                    ([320, 1600], [320, 1600])], ids=["step", "few", "many", "prompts"])
+def test_fp32_output_keeps_the_weights_in_two_parts(n, lens, dim, dtype):
+    """Whatever the size of the call, and so the kernel that runs it."""
+    pool = Pool(lens, 16, 2, dim, dtype)
+    q = torch.randn(sum(n), 16, dim, generator=torch.Generator(device="cuda").manual_seed(dim), device="cuda").to(dtype)
+    cu, kv = ints(starts(n)), ints(lens)
+    o = voxq.paged_attention(q, pool.k, pool.v, pool.table, cu, kv, max(n), max(lens), out_dtype=F32)
+    ref, _ = R.attention(q, torch.nan_to_num(pool.k), torch.nan_to_num(pool.v), pool.table, cu, kv, True, dim ** -0.5, F32)
+    assert float((R.f8(o) - ref).norm() / ref.norm()) < TWO_PARTS[dtype]

@@ -114,6 +114,16 @@ __device__ __forceinline__ uint32_t pack2v(float x, float y) {  // x in the low 
     return r;
 }
 
+// What pack2v's r leaves of x and y, in the same type.
+template <typename T>
+__device__ __forceinline__ uint32_t rest2v(uint32_t r, float x, float y) {
+    T e[2];
+    memcpy(e, &r, 4);
+    float a, b;
+    upk(fma2v(pk(to_f(e[0]), to_f(e[1])), pk(-1.0f, -1.0f), pk(x, y)), a, b);
+    return pack2v<T>(a, b);
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float x, float y) {
     if constexpr (std::is_same<T, bf16>::value) {
@@ -170,11 +180,14 @@ __device__ __forceinline__ bool next_block(const uint4* answer, int& x, int& y, 
 //                   zeroes the values past a unit's last key
 //   warp 9          issues S = Q K^T and O += P V
 //   warp 10         finds the units: this block's own, then those of blocks that have not started
-// Tensor memory: S0, S1 (128 columns each, P over their first 64), O0, O1.  The tensor pipe runs one thread's MMAs in
+// Tensor memory: S0, S1 (128 columns each, P over their first 64, its low part over the rest), O0, O1.  The tensor pipe runs one thread's MMAs in
 // order, so the S of the next key tile may follow the PV that still reads P, and a thread that has seen S complete
 // knows that every earlier PV is complete too: it may rescale O without a barrier of its own.  Rescaling is rare: sums
-// stay relative to a maximum that may be up to 2^8 behind (exact: p, l and O share it).  p is rounded to the operand
-// type, l sums the fp32 values.
+// stay relative to a maximum that may be up to 2^8 behind (exact: p, l and O share it).  l sums the fp32 values of
+// p.  For a 16-bit output p is rounded once to the operand type: that moves the output by 0.0006 of its norm in bf16, where its
+// own rounding moves it by 0.0017, and a second part takes a quarter more time (the prompts below 356 us for 285).  An fp32
+// output has no rounding to hide behind: there p enters the second product as two 16-bit parts (LOW; 305 us with one part and
+// an error of 2^-9.6 of the norm, 372 with two and under 2^-13).
 // Head dims below HD are zeros in shared memory: the tensor maps end there, and the queries are written so.  HD 256: one
 // query tile a unit and a ring of two, so that a tile's softmax waits for its products and they for it; 4 prompts of 300
 // tokens on 1000 keys 111 us, 0.2 PFLOP/s, where the MMA kernel takes 252.
@@ -187,7 +200,7 @@ __device__ __forceinline__ bool next_block(const uint4* answer, int& x, int& y, 
 // scores, read them in 70, take 1450 for maximum, exponentials (at 16 a clock an SM alone 1024 for both tiles) and
 // rounding, 220 to write the weights; a unit's output and next queries add 8500.  One or two tiles that fill the machine
 // once (3 sequences of 40..64 tokens on 12 000 keys: 37 us) pay that start and end and the join for one short run.
-template <typename T, int HD>
+template <typename T, int HD, bool LOW>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ PagedMaps maps) {
     constexpr int TILE = kTcTileBytes<HD>, ST = kTcStages<HD>, TW = kTcTiles<HD>, ROWS = TW * kTcTile;
     extern __shared__ uint8_t tc_raw[];
@@ -374,7 +387,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                             if (!ok) break;
 #pragma unroll
                             for (int j = 0; j < kTcTile / 16; j++)
-                                if (j < steps) mma_ts(tmem + 256 + t * HD, tmem + t * kTcTile + j * 8, vd + (j * 2048 >> 4), id_o, i > 0 || j > 0);
+                                if (j < steps) {
+                                    const uint32_t pt = tmem + t * kTcTile + j * 8;
+                                    if (LOW) mma_ts(tmem + 256 + t * HD, pt + kTcTile / 2, vd + (j * 2048 >> 4), id_o, i > 0 || j > 0);
+                                    mma_ts(tmem + 256 + t * HD, pt, vd + (j * 2048 >> 4), id_o, LOW || i > 0 || j > 0);
+                                }
                             if (more) {
                                 scores(t, now_k);
                             } else {
@@ -553,7 +570,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 ok = warp_wait(s_full + t, step++ & 1, VOXQ_DEVERR_WAIT_MMA, p.err);
                 if (!ok) break;
                 tc_after();
-                uint32_t sv[kTcTile];
+                uint32_t sv[kTcTile], low[LOW ? kTcTile / 2 : 1];
                 uint64_t sum[2];
                 // The weights are taken relative to the maximum so far, while this tile's maximum is found beside them:
                 // only if a row has outgrown its own by 2^8 are sums rescaled and the tile's weights computed again.
@@ -606,6 +623,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                             const int o = c - BEHIND;
                             sum[o & 1] = add2v(sum[o & 1], pk(y[2 * o], y[2 * o + 1]));
                             sv[o] = pack2v<T>(y[2 * o], y[2 * o + 1]);  // (over scores that are done with)
+                            if (LOW) low[o] = rest2v<T>(sv[o], y[2 * o], y[2 * o + 1]);
                         }
                     }
                     const float mt = top();
@@ -626,6 +644,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 }
                 tm_st32(ts, sv);
                 tm_st32(ts + 32, sv + 32);
+                if (LOW) {
+                    tm_st32(ts + 64, low);
+                    tm_st32(ts + 96, low + 32);
+                }
                 float a, b, e, f;
                 upk(sum[0], a, b);
                 upk(sum[1], e, f);
@@ -768,9 +790,9 @@ bool paged_tc_takes(const voxq_paged_attn& d) {
     return d.dtype != VOXQ_F32 && d.scale >= 0.0f && paged_maps_take(d);
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool LOW>
 static VoxCPMError tc_launch(const PagedArgs& a, cudaStream_t st) {
-    auto kern = paged_tc_kernel<T, HD>;
+    auto kern = paged_tc_kernel<T, HD, LOW>;
     static std::once_flag once;
     static cudaError_t attr = cudaSuccess;
     std::call_once(once, [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem<HD>); });
@@ -784,6 +806,11 @@ static VoxCPMError tc_launch(const PagedArgs& a, cudaStream_t st) {
     const dim3 grid(d.batch <= 32 * kTcSeqs ? (int)paged_tiles(d, rows) : ((int)((int64_t)d.total_q * a.group / rows) + d.batch) * d.kv_heads, 1, a.splits);
     VOXQ_CUDA_TRY(launch_pdl(kern, grid, dim3(kTcThreads), kTcSmem<HD>, st, a, m));
     return VOXCPM_SUCCESS;
+}
+
+template <typename T, int HD>
+static VoxCPMError tc_launch(const PagedArgs& a, cudaStream_t st) {
+    return a.d.out_dtype == VOXQ_F32 ? tc_launch<T, HD, true>(a, st) : tc_launch<T, HD, false>(a, st);
 }
 
 VoxCPMError paged_tc_launch(const PagedArgs& a, cudaStream_t st) {

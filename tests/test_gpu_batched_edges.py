@@ -30,3 +30,21 @@ def test_fp32_output_keeps_the_weights_in_two_parts(n, lens, dim, dtype):
     o = voxq.paged_attention(q, pool.k, pool.v, pool.table, cu, kv, max(n), max(lens), out_dtype=F32)
     ref, _ = R.attention(q, torch.nan_to_num(pool.k), torch.nan_to_num(pool.v), pool.table, cu, kv, True, dim ** -0.5, F32)
     assert float((R.f8(o) - ref).norm() / ref.norm()) < TWO_PARTS[dtype]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=ids)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_many_units_of_one_key_tile_with_odd_ends(dim, dtype):
+    """Every unit of work is one tile of keys that ends inside 16 of them, so that its loader runs furthest ahead of its
+    products: the same bits every time, no wait that gives up, and the right ones."""
+    n = [16 + i % 3 for i in range(600)]
+    lens = [a + 17 + 2 * (i % 40) for i, a in enumerate(n)]
+    pool = Pool(lens, 16, 2, dim, dtype)
+    q = torch.randn(sum(n), 16, dim, device="cuda").to(dtype)
+    cu, kv = ints(starts(n)), ints(lens)
+    outs = [voxq.paged_attention(q, pool.k, pool.v, pool.table, cu, kv, max(n), max(lens)) for _ in range(20)]
+    assert all(torch.equal(outs[0], o) for o in outs) and int(voxq.lib().voxq_device_error(1)) == 0
+    some = 40
+    ref, bound = R.attention(q[:cu[some]], torch.nan_to_num(pool.k), torch.nan_to_num(pool.v), pool.table[:some], cu[:some + 1],
+                             kv[:some], True, dim ** -0.5)
+    R.assert_within(outs[0][:cu[some]], ref, bound)

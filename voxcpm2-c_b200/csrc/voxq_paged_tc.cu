@@ -16,6 +16,10 @@ constexpr int kTcTiles = HD > 128 ? 1 : 2;   // query tiles of a unit: tensor me
 template <int HD>
 constexpr int kTcStages = HD > 128 ? 2 : 5;  // ring of key and value tiles
 constexpr int kTcHalf = kTcTile * 128;       // bytes of 128 rows x 64 dims, 128-byte-swizzled rows
+// Barriers of the mended ends of units, in turn.  Before the MMA warp waits for a unit's it has freed that unit's last key tile but
+// not its last value tile, so of a ring of five the loader can have mended that unit's end and two more (units of one tile
+// each: V K V K V), never a fourth, and a barrier's phase is seen before its next one begins.
+constexpr int kTcTails = 3;
 constexpr int kTcItems = 4;                  // units in flight between the warps of a block
 constexpr int kTcSeqs = 4;                   // of 32 sequences: up to how many the units are taken in order of their keys
 constexpr uint32_t kTcLong = 20000;           // limit (ms) of the waits that span a whole unit of work
@@ -203,15 +207,16 @@ __device__ __forceinline__ bool next_block(const uint4* answer, int& x, int& y, 
 template <typename T, int HD, bool LOW>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ PagedMaps maps) {
     constexpr int TILE = kTcTileBytes<HD>, ST = kTcStages<HD>, TW = kTcTiles<HD>, ROWS = TW * kTcTile;
+    static_assert(ST < 2 * kTcTails, "as many mended ends as the ring can hold");
     extern __shared__ uint8_t tc_raw[];
-    __shared__ uint64_t bar[2 * ST + 2 * kTcItems + 12];
+    __shared__ uint64_t bar[2 * ST + 2 * kTcItems + 10 + kTcTails];
     __shared__ uint4 answer;
     __shared__ TcItem items[kTcItems];
     __shared__ uint32_t tmem_slot;
     uint64_t *full = bar, *empty = full + ST;                                // ring
     uint64_t *s_full = empty + ST, *p_full = s_full + 2;  // per query tile
     uint64_t *o_done = p_full + 2, *q_full = o_done + 2;
-    uint64_t *item_full = q_full + 2, *item_empty = item_full + kTcItems, *tail = item_empty + kTcItems, *asked = tail + 2, *begun = asked + 1;
+    uint64_t *item_full = q_full + 2, *item_empty = item_full + kTcItems, *tail = item_empty + kTcItems, *asked = tail + kTcTails, *begun = asked + 1;
     const voxq_paged_attn& d = p.d;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, G = p.group;
     const uint32_t qsm = (smem_u32(tc_raw) + 1023) & ~1023u, ring = qsm + TW * TILE;
@@ -226,8 +231,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             mbar_init(p_full + i, 4);
             mbar_init(o_done + i, 1);
             mbar_init(q_full + i, 4);
-            mbar_init(tail + i, 1);  // (in turn: the ring holds at most two units' ends ahead of the MMA warp)
         }
+        for (int i = 0; i < kTcTails; i++) mbar_init(tail + i, 1);
         for (int i = 0; i < kTcItems; i++) {
             mbar_init(item_full + i, 1);
             mbar_init(item_empty + i, 10);  // every warp that works on units
@@ -307,7 +312,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(tail + (tails & 1));
+                    if (lane == 0) mbar_arrive(tail + tails % kTcTails);
                     tails++;
                 }
             }
@@ -369,7 +374,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                             sk = slot;
                             advance();
                         } else if (odd) {
-                            ok = ok && mbar_wait_bounded(tail + (tails & 1), (tails >> 1) & 1, VOXQ_DEVERR_WAIT_FULL, p.err);
+                            ok = ok && mbar_wait_bounded(tail + tails % kTcTails, (tails / kTcTails) & 1, VOXQ_DEVERR_WAIT_FULL, p.err);
                             tails++;
                         }
                     };

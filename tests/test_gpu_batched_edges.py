@@ -1,6 +1,8 @@
 """The batched-step operators on the GPU where types, sizes and values meet their limits."""
 from __future__ import annotations
 
+import ctypes as C
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -48,3 +50,31 @@ def test_many_units_of_one_key_tile_with_odd_ends(dim, dtype):
     ref, bound = R.attention(q[:cu[some]], torch.nan_to_num(pool.k), torch.nan_to_num(pool.v), pool.table[:some], cu[:some + 1],
                              kv[:some], True, dim ** -0.5)
     R.assert_within(outs[0][:cu[some]], ref, bound)
+
+
+@pytest.mark.parametrize("D", [8, 16, 24, 32, 48])
+@pytest.mark.parametrize("H,KVH", [(1, 1), (2, 1), (1, 0), (2, 0), (0, 1)])
+@pytest.mark.parametrize("rotate", [True, False], ids=["rot", "plain"])
+def test_rope_append_of_few_small_heads(H, KVH, D, rotate):
+    """So little a token that more tokens would fit a block than a block may have along one of its axes.  From C, where
+    queries or the cache may be left out."""
+    T, pages, page = 150, 21, 8
+    qkv = torch.randn(T, H + 2 * KVH, D, device="cuda")
+    q, k, v = qkv[:, :H], qkv[:, H:H + KVH], qkv[:, H + KVH:]
+    out, ck, cv = torch.zeros(T, H, D, device="cuda"), *(torch.zeros(pages, page, KVH, D, device="cuda") for _ in range(2))
+    freqs, pos = voxq.rope_freqs(200, D), ints(range(T))
+    slot = torch.randperm(pages * page, device="cuda")[:T]
+    row = (H + 2 * KVH) * D
+    d = voxq.RopeDesc(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride=row, q_head_stride=D, k_stride=row, k_head_stride=D,
+                      v_stride=row, v_head_stride=D, q_out=out.data_ptr() if H else None, qo_stride=H * D, qo_head_stride=D,
+                      cache_k=ck.data_ptr(), cache_v=cv.data_ptr(), page_stride=page * KVH * D, row_stride=KVH * D, head_stride=D,
+                      freqs=freqs.data_ptr() if rotate else None, positions=pos.data_ptr(), slots=slot.data_ptr(), tokens=T, heads=H,
+                      kv_heads=KVH, head_dim=D, rot_dim=D if rotate else 0, n_pos=200, pages=pages, page_size=page,
+                      in_dtype=voxq.F32, cache_dtype=voxq.F32)
+    voxq.check(voxq.lib().voxq_rope_append(C.byref(d), torch.cuda.current_stream().cuda_stream), "voxq_rope_append")
+    turned = lambda x: R.rotate(x, freqs, pos, False, F32) if rotate else (R.f8(x), 0 * R.f8(x))  # noqa: E731
+    if H:
+        R.assert_within(out, *turned(q), "q")
+    if KVH:
+        R.assert_within(ck.flatten(0, 1)[slot], *turned(k), "k")
+        assert torch.equal(cv.flatten(0, 1)[slot], v)

@@ -157,7 +157,7 @@ template <typename T, typename C, int CH>
 static cudaError_t rope_launch(const voxq_rope& p, cudaStream_t st) {
     const int items = p.head_dim / (2 * CH), heads = p.heads + 2 * p.kv_heads;
     const int y = std::min(heads, std::max(1, kRopeThreads / items));
-    const int z = std::max(1, kRopeThreads / (items * y));
+    const int z = std::min(64, std::max(1, kRopeThreads / (items * y)));  // 64: a block's limit along z
     auto kern = p.interleaved ? rope_append_kernel<T, C, CH, true> : rope_append_kernel<T, C, CH, false>;
     return launch_pdl(kern, dim3((p.tokens + z - 1) / z), dim3(items, y, z), 0, st, p);
 }

@@ -525,7 +525,7 @@ typedef struct {
     double attn_factor;            /* 0 -> 1 */
     int32_t original_len;          /* VOXQ_ROPE_YARN */
     const double* long_factors;    /* VOXQ_ROPE_LONG: host [rot_dim / 2], read before the call returns; rot_dim <= 256 */
-    float* out;                    /* [n_pos][rot_dim / 2][2] */
+    float* out;                    /* [n_pos][rot_dim / 2][2], 8-byte aligned */
 } voxq_rope_table;
 VOXQ_API VoxCPMError voxq_rope_freqs(const voxq_rope_table* d, void* stream);
 
@@ -548,7 +548,7 @@ typedef struct {
     int64_t qo_stride, qo_head_stride;
     void *cache_k, *cache_v;              /* [pages][page_size][kv_heads][head_dim], the same strides for both */
     int64_t page_stride, row_stride, head_stride;
-    const float* freqs;                   /* [n_pos][rot_dim / 2][2]; NULL: no rotation (rot_dim 0) */
+    const float* freqs;                   /* [n_pos][rot_dim / 2][2], 8-byte aligned; NULL: no rotation (rot_dim 0) */
     const int32_t* positions;             /* [tokens], clamped to [0, n_pos) */
     const int64_t* slots;                 /* [tokens] */
     int32_t tokens, heads, kv_heads, head_dim, rot_dim, interleaved, n_pos;

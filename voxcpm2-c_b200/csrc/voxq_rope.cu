@@ -176,6 +176,7 @@ extern "C" VoxCPMError voxq_rope_freqs(const voxq_rope_table* d, void* stream) {
     if (d->scaling == VOXQ_ROPE_NTK && d->rot_dim == 2) return VOXCPM_ERR_SHAPE_MISMATCH;
     if (d->scaling == VOXQ_ROPE_YARN && d->original_len <= 0) return VOXCPM_ERR_SHAPE_MISMATCH;
     if (d->scaling == VOXQ_ROPE_LONG && !d->long_factors) return VOXCPM_ERR_INTERNAL;
+    if ((uintptr_t)d->out & 7) return VOXCPM_ERR_UNSUPPORTED;  // pairs in one access
     if (d->n_pos == 0 || d->rot_dim == 0) return VOXCPM_SUCCESS;
     RopeFreqs p{};
     p.out = d->out;
@@ -229,6 +230,7 @@ extern "C" VoxCPMError voxq_rope_append(const voxq_rope* d, void* stream) {
     if (d->tokens == 0 || d->head_dim == 0 || (heads == 0 && !store)) return VOXCPM_SUCCESS;
     if ((turn && !d->positions) || (heads && !d->q) || (store && (!d->k || !d->v || !d->cache_k || !d->cache_v || !d->slots)))
         return VOXCPM_ERR_INTERNAL;
+    if (turn && ((uintptr_t)d->freqs & 7)) return VOXCPM_ERR_UNSUPPORTED;  // pairs in one access
     const int it = d->in_dtype, ct = d->cache_dtype;
     if (heads && !(rows16(d->q, d->q_stride, it) && rows16(d->q, d->q_head_stride, it) && rows16(d->q_out, d->qo_stride, ct) &&
                    rows16(d->q_out, d->qo_head_stride, ct)))

@@ -629,8 +629,8 @@ VOXQ_API VoxCPMError voxq_lora_forward(const voxq_lora* d, void* stream);
  * gate_index[m] clamped to [0, gate_rows), or, with gate_index NULL, m when
  * gate_rows == rows and 0 when gate_rows == 1.  h_out may be x or y, n_out may be y or x (not both one buffer).
  * y, x, gate, h_out and n_out are one type, the norm weights
- * fp32.  Any D from 1 to 16384 and any alignment (16-byte rows take wide
- * loads). */
+ * fp32.  Any D from 1 to 16384 and any alignment down to an element's own
+ * (16-byte rows take wide loads). */
 typedef struct {
     const void *y, *x, *gate;
     int64_t ldy, ldx, ldg;

@@ -211,6 +211,7 @@ extern "C" VoxCPMError voxq_norm_residual(const voxq_norm* d, void* stream) {
         return d->D % v == 0 && rows(d->y, d->ldy) && rows(d->x, d->ldx) && rows(d->gate, d->ldg) && rows(d->h_out, d->ldh) &&
                rows(d->n_out, d->ldn) && weights(d->w_post) && weights(d->w_pre);
     };
+    if (!fits(1)) return VOXCPM_ERR_UNSUPPORTED;  // elements themselves out of line
     const int wide = 16 / elem_bytes(dt), width = fits(wide) ? wide : fits(2) ? 2 : 1;
     VOXQ_CUDA_TRY(with_elem(dt, [&](auto x) { return norm_dispatch<decltype(x)>(*d, width, (cudaStream_t)stream); }));
     return VOXCPM_SUCCESS;

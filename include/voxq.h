@@ -131,7 +131,8 @@ VOXQ_API const char* voxq_version(void);
  * the kernels that need more than 48 KB of shared memory get their opt-in on
  * the first device that launches them in a process, so one process drives one
  * GPU (a launch on a second device returns VOXCPM_ERR_INTERNAL); run one
- * process per GPU, as bench.py and the serving workers do. */
+ * process per GPU, as bench.py and the serving workers do.  The operators of a
+ * batched step (below) ask on every device. */
 VOXQ_API VoxCPMError voxq_set_device(int device);
 
 /* Device-side status of the current device's kernels: 0, or the code of the

@@ -2,12 +2,14 @@
 from __future__ import annotations
 
 import ctypes as C
+import os
+import subprocess
 
 import pytest
 
 torch = pytest.importorskip("torch")
 import voxq  # noqa: E402
-from test_batched_cpu import P, norm, rope  # noqa: E402
+from test_batched_cpu import P, REPO, norm, rope  # noqa: E402
 
 
 @pytest.mark.parametrize("off", [1, 2, 4, 12])
@@ -24,3 +26,33 @@ def test_norm_rows_between_elements_are_refused():
     for kw in (dict(y=P + 1), dict(x=P + 2), dict(n_out=P + 3), dict(w_pre=P + 2), dict(w_post=P + 1), dict(gate=P + 2, gate_rows=1, ldg=64)):
         assert L.voxq_norm_residual(C.byref(norm(**kw)), None) == voxq.UNSUPPORTED, kw
     assert L.voxq_norm_residual(C.byref(norm(dtype=voxq.F16, h_out=P + 1)), None) == voxq.UNSUPPORTED
+
+
+def test_shared_memory_is_asked_for_on_every_device(tmp_path):
+    """allow_shared against a stand-in runtime: once a device, again after a failure."""
+    src = tmp_path / "t.cpp"
+    src.write_text(r'''
+#include "voxq_internal.h"
+static int dev, calls, fail;
+extern "C" cudaError_t cudaGetDevice(int* d) { *d = dev; return cudaSuccess; }
+extern "C" cudaError_t cudaFuncSetAttribute(const void*, cudaFuncAttribute, int) {
+    calls++;
+    return fail ? cudaErrorInvalidValue : cudaSuccess;
+}
+int main() {
+    std::atomic<uint64_t> asked{0};
+    auto ask = [&](int d, int f) { dev = d; fail = f; return voxq::allow_shared(nullptr, 100000, asked); };
+    if (ask(0, 1) == cudaSuccess || calls != 1) return 1;
+    if (ask(0, 0) != cudaSuccess || calls != 2) return 2;
+    if (ask(0, 1) != cudaSuccess || calls != 2) return 3;
+    if (ask(1, 0) != cudaSuccess || calls != 3) return 4;
+    if (ask(63, 0) != cudaSuccess || ask(63, 1) != cudaSuccess || calls != 4) return 5;
+    if (ask(64, 0) != cudaSuccess || ask(64, 0) != cudaSuccess || calls != 6) return 6;
+    return 0;
+}
+''')
+    exe = tmp_path / "t"
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc"))), "include")
+    subprocess.run(["g++", "-std=c++17", "-I", os.path.join(REPO, "include"), "-I", os.path.join(REPO, "voxcpm2-c_b200", "csrc"), "-I", cuda,
+                    str(src), "-o", str(exe)], check=True)
+    assert subprocess.run([str(exe)]).returncode == 0

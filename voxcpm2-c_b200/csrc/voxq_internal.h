@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "voxq.h"
 
 namespace voxq {
@@ -42,6 +44,19 @@ VoxCPMError dense_launch(const float* a, int M, int64_t lda, const void* w, int 
 
 // fp16 -> fp32, exact (voxq_dense.cu).
 VoxCPMError widen_fp16(const uint16_t* src, float* dst, size_t n, cudaStream_t st);
+
+// Lets a kernel take `bytes` of dynamic shared memory on the current device.  The attribute is a device's, so it is asked
+// for once on each; `asked` is the kernel's own (a bit for a device), and keeps no failed attempt.
+inline cudaError_t allow_shared(const void* kern, int bytes, std::atomic<uint64_t>& asked) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+    if (asked.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 // Per-device device-side error word (allocated on first use, zeroed).
 int* device_error_word();

@@ -1,6 +1,5 @@
 // voxq_lora.cu -- low-rank adapters of many requests beside a shared projection.
 #include <algorithm>
-#include <mutex>
 #include <type_traits>
 
 #include "voxq_batch.cuh"
@@ -329,13 +328,9 @@ template <typename T, typename W, int TM, int RB, int COLS>
 static VoxCPMError lora_launch(const voxq_lora& d, cudaStream_t st) {
     using S = LoraShape<T, W, TM, COLS>;
     const S z(d.rank);
-    static std::once_flag once;
-    static cudaError_t attr = cudaSuccess;
     auto kern = lora_kernel<T, W, TM, RB, COLS>;
-    std::call_once(once, [&] {
-        attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S(RB * 8).bytes);
-    });
-    VOXQ_CUDA_TRY(attr);
+    static std::atomic<uint64_t> asked{0};
+    VOXQ_CUDA_TRY(allow_shared((const void*)kern, S(RB * 8).bytes, asked));
     // As many CTAs to a tile as keep the grid within 4 an SM, up to 8.  Where 4 fit an SM any number, else a power of two, which
     // leaves no holes in a second round.  bf16 prompts (8000 rows, K 1024, N 4096, rank 32): 42 us, 47 with powers of two, 71
     // with a bound of 2 an SM and 50 with 8; 9 of 1000 rows, rank 64, K 2960, N 1032: 59 us, 78 with any number.

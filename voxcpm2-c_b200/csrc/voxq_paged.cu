@@ -2,7 +2,6 @@
 #include <math.h>
 
 #include <algorithm>
-#include <mutex>
 
 #include "voxq_internal.h"
 #include "voxq_paged.cuh"
@@ -309,10 +308,8 @@ template <typename T, int HD>
 static VoxCPMError paged_mma_launch(const PagedArgs& a, cudaStream_t st) {
     using S = PagedShape<T, HD>;
     auto kern = paged_mma_kernel<T, HD>;
-    static std::once_flag once;
-    static cudaError_t attr = cudaSuccess;
-    std::call_once(once, [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes); });
-    VOXQ_CUDA_TRY(attr);
+    static std::atomic<uint64_t> asked{0};
+    VOXQ_CUDA_TRY(allow_shared((const void*)kern, S::bytes, asked));
     const dim3 grid((int)((int64_t)a.d.total_q * a.group / S::TR) + a.d.batch, a.d.kv_heads, a.splits);
     VOXQ_CUDA_TRY(launch_pdl(kern, grid, dim3(kMmaThreads), S::bytes, st, a));
     return VOXCPM_SUCCESS;

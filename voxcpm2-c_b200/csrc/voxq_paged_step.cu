@@ -1,6 +1,5 @@
 // voxq_paged_step.cu -- paged attention of at most 16 rows a sequence and kv head: the next-token step.
 #include <algorithm>
-#include <mutex>
 
 #include "voxq_internal.h"
 #include "voxq_paged.cuh"
@@ -413,10 +412,8 @@ template <typename T, int HD>
 static VoxCPMError step_launch(const PagedArgs& a, cudaStream_t st) {
     using S = StepShape<T, HD>;
     auto kern = paged_step_kernel<T, HD>;
-    static std::once_flag once;
-    static cudaError_t attr = cudaSuccess;
-    std::call_once(once, [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes); });
-    VOXQ_CUDA_TRY(attr);
+    static std::atomic<uint64_t> asked{0};
+    VOXQ_CUDA_TRY(allow_shared((const void*)kern, S::bytes, asked));
     PagedMaps m;
     const VoxCPMError e = paged_maps(a.d, S::KT, &m);
     if (e != VOXCPM_SUCCESS) return e;

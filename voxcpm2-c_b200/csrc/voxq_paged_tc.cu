@@ -798,10 +798,8 @@ bool paged_tc_takes(const voxq_paged_attn& d) {
 template <typename T, int HD, bool LOW>
 static VoxCPMError tc_launch(const PagedArgs& a, cudaStream_t st) {
     auto kern = paged_tc_kernel<T, HD, LOW>;
-    static std::once_flag once;
-    static cudaError_t attr = cudaSuccess;
-    std::call_once(once, [&] { attr = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem<HD>); });
-    VOXQ_CUDA_TRY(attr);
+    static std::atomic<uint64_t> asked{0};
+    VOXQ_CUDA_TRY(allow_shared((const void*)kern, kTcSmem<HD>, asked));
     const voxq_paged_attn& d = a.d;
     PagedMaps m;
     const VoxCPMError e = paged_maps(d, kTcTile, &m);

@@ -56,3 +56,37 @@ int main() {
     subprocess.run(["g++", "-std=c++17", "-I", os.path.join(REPO, "include"), "-I", os.path.join(REPO, "voxcpm2-c_b200", "csrc"), "-I", cuda,
                     str(src), "-o", str(exe)], check=True)
     assert subprocess.run([str(exe)]).returncode == 0
+
+
+def test_tensors_of_several_gpus_are_refused():
+    """Each call with one of its tensors on a second GPU, the others on the first (fake tensors: shapes and devices without
+    memory, so nothing can be launched)."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    i32, i64 = torch.int32, torch.int64
+    calls = {
+        voxq.paged_attention: [((1, 4, 64),), ((2, 16, 2, 64),), ((2, 16, 2, 64),), ((1, 2), i32), ((2,), i32), ((1,), i32), 1, 16, True, 0.0, ((1, 4, 64),)],
+        voxq.rope_append: [((1, 4, 64),), ((1, 2, 64),), ((1, 2, 64),), ((8, 32, 2),), ((1,), i32), ((1,), i64), ((2, 16, 2, 64),), ((2, 16, 2, 64),), ((1, 4, 64),)],
+        voxq.lora: [((2, 64),), ((1, 8, 64),), ((1, 32, 8),), ((2,), i32), ((1,), i32), ((1,),), ((2, 32),), ((2, 32),), ((1,), i32)],
+        voxq.norm_residual: [((2, 64),), ((2, 64),), ((64,),), ((64,),), ((3, 64),), ((2,), i32), 1.0, 1e-5, ((2, 64),), ((2, 64),)],
+    }
+    with FakeTensorMode():
+        for f, spec in calls.items():
+            for away in [i for i, s in enumerate(spec) if isinstance(s, tuple)]:
+                args = [s if not isinstance(s, tuple) else
+                        torch.empty(s[0], dtype=s[1] if len(s) > 1 else torch.float32, device=f"cuda:{int(i == away)}") for i, s in enumerate(spec)]
+                with pytest.raises(ValueError, match="one GPU"):
+                    f(*args)
+
+
+def test_streams_of_another_gpu_are_refused():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    class Stream:
+        cuda_stream, device = 0, torch.device("cuda:1")
+
+    with FakeTensorMode():
+        y = torch.empty(2, 64, device="cuda:0")
+        with pytest.raises(ValueError, match="stream"):
+            voxq.norm_residual(y, y, stream=Stream())
+    with pytest.raises(ValueError):
+        voxq.norm_residual(torch.zeros(2, 64), torch.zeros(2, 64), stream=Stream())

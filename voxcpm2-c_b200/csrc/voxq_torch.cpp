@@ -4,11 +4,13 @@
 // tensors and packing a descriptor from Python took 8 more.  Here that is 1 to 2.  The functions take positional
 // arguments from batched.py's wrappers (which document them), check them, make missing outputs on the current stream and
 // call libvoxq's entry points, whose addresses `bind` gets from the ctypes binding.  A tensor that does not fit raises
-// ValueError; a code from the library raises VoxqError.
+// ValueError; a code from the library raises VoxqError.  A call's tensors are on one GPU, which is made the current one for
+// it: kernels, plans and the library's status word belong to the current device, the stream to the tensors'.
 #include <Python.h>
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -62,6 +64,10 @@ int code_of(at::ScalarType t) {
 bool rows_ok(const at::Tensor& t, int64_t dims) {
     return t.dim() == dims && t.is_cuda() && (t.stride(-1) == 1 || t.size(-1) <= 1);
 }
+// tensors (or nullptr) on the device of `like`
+void beside(const at::Tensor& like, std::initializer_list<const at::Tensor*> others) {
+    for (const at::Tensor* t : others) need(!t || t->device() == like.device(), "all tensors of a call are needed on one GPU");
+}
 // a contiguous device vector of n values
 const void* vec(const at::Tensor& t, int64_t n, at::ScalarType type, const char* what) {
     need(t.scalar_type() == type && t.numel() == n && t.is_cuda() && t.is_contiguous(), what);
@@ -89,8 +95,8 @@ int i32(int64_t v) {
 void* stream_of(const at::Tensor& like) { return (void*)c10::cuda::getCurrentCUDAStream(like.get_device()).stream(); }
 
 // Memory of the current stream, contiguous, without the dispatcher's half microsecond a tensor.
-at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& beside) {
-    return at::detail::empty_cuda(sizes, type, beside.device(), std::nullopt);
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+    return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
 }
 
 template <typename F>
@@ -120,19 +126,22 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor &q = present(a[0], "q: a tensor is needed"), &k = present(a[1], "k: a tensor is needed"), &v = present(a[2], "v: a tensor is needed");
         const at::Tensor *freqs = tensor(a[3], "freqs: a tensor is needed"), &slots = present(a[5], "slots: a tensor is needed");
         const at::Tensor &ck = present(a[6], "cache_k: a tensor is needed"), &cv = present(a[7], "cache_v: a tensor is needed"), *given = tensor(a[8], "q_out: a tensor is needed");
+        const at::Tensor* positions = freqs ? &present(a[4], "positions: a tensor is needed") : nullptr;
         need(rows_ok(q, 3) && rows_ok(k, 3) && rows_ok(v, 3), "q, k, v: 3-dimensional CUDA tensors with a contiguous last dimension are needed");
+        beside(q, {&k, &v, freqs, positions, &slots, &ck, &cv, given});
         const int64_t T = q.size(0), H = q.size(1), D = q.size(2), KVH = k.size(1);
         need(v.sizes() == k.sizes() && k.size(0) == T && k.size(2) == D && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
              "q [T, heads, D] and k, v [T, kv_heads, D] of one type are needed");
         caches(ck, cv, D);
         need(ck.size(2) == KVH, "the caches' kv_heads differ from k's");
+        const c10::cuda::CUDAGuard here(q.device());
         at::Tensor out = given ? *given : fresh(q.sizes(), ck.scalar_type(), q);
         need(rows_ok(out, 3) && out.sizes() == q.sizes() && out.scalar_type() == ck.scalar_type(), "q_out: q's shape and the caches' type, on the GPU");
         voxq_rope d{};
         if (freqs) {
             need(freqs->dim() == 3 && freqs->size(2) == 2, "freqs: [n_pos, rot / 2, 2]");
             d.freqs = (const float*)vec(*freqs, freqs->numel(), at::kFloat, "freqs: a contiguous fp32 CUDA tensor is needed");
-            d.positions = (const int32_t*)vec(present(a[4], "positions: a tensor is needed"), T, at::kInt, "positions: a contiguous CUDA vector of int32, one per token");
+            d.positions = (const int32_t*)vec(*positions, T, at::kInt, "positions: a contiguous CUDA vector of int32, one per token");
             d.n_pos = i32(freqs->size(0));
             d.rot_dim = i32(2 * freqs->size(1));
         }
@@ -175,6 +184,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor &bt = present(a[3], "block_table: a tensor is needed"), &cu = present(a[4], "cu_q: a tensor is needed"), &kv = present(a[5], "kv_len: a tensor is needed");
         const at::Tensor* given = tensor(a[10], "out: a tensor is needed");
         need(rows_ok(q, 3), "q: a 3-dimensional CUDA tensor with a contiguous last dimension is needed");
+        beside(q, {&ck, &cv, &bt, &cu, &kv, given});
         caches(ck, cv, q.size(2));
         const int64_t B = kv.numel();
         need(rows_ok(bt, 2) && bt.size(0) == B && bt.scalar_type() == at::kInt && ck.scalar_type() == q.scalar_type(),
@@ -183,6 +193,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         d.max_q = as_i32(a[6], "max_q is past 2^31");
         d.max_kv = as_i32(a[7], "max_kv is past 2^31");
         need(d.max_kv <= bt.size(1) * ck.size(1), "max_kv is more than the block table's pages hold");
+        const c10::cuda::CUDAGuard here(q.device());
         at::Tensor out = given ? *given : fresh(q.sizes(), q.scalar_type(), q);
         need(rows_ok(out, 3) && out.sizes() == q.sizes(), "out: q's shape, contiguous along head_dim, on the GPU");
         d.q = q.const_data_ptr();
@@ -230,12 +241,14 @@ PyObject* lora(PyObject*, PyObject* const* o, Py_ssize_t n) {
         const at::Tensor &cu = present(o[3], "cu: a tensor is needed"), &who = present(o[4], "adapter: a tensor is needed"), &scale = present(o[5], "scale: a tensor is needed");
         const at::Tensor *base = tensor(o[6], "base: a tensor is needed"), *given = tensor(o[7], "out: a tensor is needed"), *ranks = tensor(o[8], "ranks: a tensor is needed");
         need(rows_ok(x, 2), "x: a 2-dimensional CUDA tensor with a contiguous last dimension is needed");
+        beside(x, {&a, &b, &cu, &who, &scale, base, given, ranks});
         need(a.dim() == 3 && b.dim() == 3 && a.size(2) == x.size(1) && b.size(0) == a.size(0) && b.size(2) == a.size(1) &&
                  a.scalar_type() == b.scalar_type() && a.is_contiguous() && b.is_contiguous() && a.is_cuda() && b.is_cuda(),
              "contiguous CUDA a [adapters, rank, K] and b [adapters, N, rank] of one type are needed");
         const int64_t M = x.size(0), N = b.size(1), B = who.numel(), nA = a.size(0);
         auto fits = [&](const at::Tensor& t) { return rows_ok(t, 2) && t.size(0) == M && t.size(1) == N && t.scalar_type() == x.scalar_type(); };
         need(!base || fits(*base), "base: [rows, N] of x's type, contiguous along N, on the GPU");
+        const c10::cuda::CUDAGuard here(x.device());
         at::Tensor out = given ? *given : fresh({M, N}, x.scalar_type(), x);
         need(fits(out), "out: [rows, N] of x's type, contiguous along N, on the GPU");
         voxq_lora d{};
@@ -274,10 +287,12 @@ PyObject* norm_residual(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor *gate = tensor(a[4], "gate: a tensor is needed"), *index = tensor(a[5], "gate_index: a tensor is needed");
         const at::Tensor *h_given = tensor(a[8], "h_out: a tensor is needed"), *n_given = tensor(a[9], "n_out: a tensor is needed");
         need(rows_ok(y, 2), "y: a 2-dimensional CUDA tensor with a contiguous last dimension is needed");
+        beside(y, {&x, w_pre, w_post, gate, index, h_given, n_given});
         auto fits = [&](const at::Tensor& t) { return rows_ok(t, 2) && t.sizes() == y.sizes() && t.scalar_type() == y.scalar_type(); };
         need(fits(x), "y and x: [rows, D] of one type, contiguous along D, on the GPU");
         need(w_pre || !n_given, "n_out needs w_pre");
         const int64_t M = y.size(0), D = y.size(1);
+        const c10::cuda::CUDAGuard here(y.device());
         voxq_norm d{};
         if (gate) {
             need(rows_ok(*gate, 2) && gate->size(1) == D && gate->scalar_type() == y.scalar_type(),

@@ -25,10 +25,19 @@ def _need(ok, what):
         raise ValueError(what)
 
 
-def _on(stream):
-    """Makes `stream` the current one: outputs and workspaces that a call makes then belong to it, and are not handed
-    out again while the call uses them."""
-    return torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream)))
+def _on(stream, device):
+    """Makes `stream` the current one of `device`: outputs and workspaces that a call makes then belong to it, and are
+    not handed out again while the call uses them."""
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream), device=device)
+    _need(stream.device == device, f"a stream of {stream.device} for tensors on {device}")
+    return torch.cuda.stream(stream)
+
+
+def _device(t):
+    """Where a call runs: its first tensor's GPU."""
+    _need(isinstance(t, torch.Tensor) and t.is_cuda, "a CUDA tensor is needed")
+    return t.device
 
 
 def rope_freqs(n_pos: int, rot_dim: int, theta: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
@@ -41,16 +50,19 @@ def rope_freqs(n_pos: int, rot_dim: int, theta: float = 10000.0, scaling: Option
     _need(scaling != "long" or (long_factors is not None and len(long_factors) == rot_dim // 2),
           "long scaling needs rot_dim / 2 factors")
     if stream is not None:
-        with _on(stream):
+        device = torch.empty(0, device=device).device
+        with _on(stream, device):
             return rope_freqs(n_pos, rot_dim, theta, scaling, factor, original_len, beta_fast, beta_slow, attn_factor,
                               long_factors, device)
     out = torch.empty((n_pos, rot_dim // 2, 2), dtype=torch.float32, device=device)
     if out.numel() == 0:
         return out
+    _need(out.is_cuda, "device: a GPU is needed")
     lf = (C.c_double * len(long_factors))(*long_factors) if scaling == "long" else None
     d = RopeTableDesc(n_pos, rot_dim, ROPE_SCALING[scaling], theta, factor, beta_fast, beta_slow, attn_factor,
                       original_len, C.cast(lf, C.c_void_p) if lf is not None else None, out.data_ptr())
-    check(lib().voxq_rope_freqs(C.byref(d), torch.cuda.current_stream(out.device).cuda_stream), "voxq_rope_freqs")
+    with torch.cuda.device(out.device):
+        check(lib().voxq_rope_freqs(C.byref(d), torch.cuda.current_stream().cuda_stream), "voxq_rope_freqs")
     return out
 
 
@@ -62,7 +74,7 @@ def rope_append(q, k, v, freqs, positions, slots, cache_k, cache_v, q_out=None, 
     queries in the caches' type.  q [T, heads, D]; k, v [T, kv_heads, D]; freqs [n_pos, rot / 2, 2] (None: no
     rotation); positions int32 [T]; slots int64 [T], page * page_size + offset, -1 for padding rows."""
     if stream is not None:
-        with _on(stream):
+        with _on(stream, _device(q)):
             return rope_append(q, k, v, freqs, positions, slots, cache_k, cache_v, q_out, interleaved)
     return _torch.rope_append(q, k, v, freqs, positions, slots, cache_k, cache_v, q_out, interleaved)
 
@@ -74,7 +86,7 @@ def paged_attention(q, cache_k, cache_v, block_table, cu_q, kv_len, max_q: int, 
     int32 [batch], the new tokens included; max_q, max_kv: upper bounds of both.  scale 0: 1 / sqrt(D).  out_dtype:
     q's type (default) or torch.float32."""
     if stream is not None:
-        with _on(stream):
+        with _on(stream, _device(q)):
             return paged_attention(q, cache_k, cache_v, block_table, cu_q, kv_len, max_q, max_kv, causal, scale, out, out_dtype)
     if out is None and out_dtype is not None:
         out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
@@ -86,7 +98,7 @@ def lora(x, a, b, cu, adapter, scale, base=None, out=None, ranks=None, stream=No
     x [rows, K]; a [adapters, rank, K]; b [adapters, N, rank]; cu int32 [batch + 1]; adapter int32 [batch], -1 for
     none; scale fp32 [adapters]; ranks int32 [adapters] or None; base [rows, N] or None; out may be base."""
     if stream is not None:
-        with _on(stream):
+        with _on(stream, _device(x)):
             return lora(x, a, b, cu, adapter, scale, base, out, ranks)
     return _torch.lora(x, a, b, cu, adapter, scale, base, out, ranks)
 
@@ -97,6 +109,6 @@ def norm_residual(y, x, w_pre=None, w_post=None, gate=None, gate_index=None, alp
     n is None without w_pre).  y, x [rows, D]; norm weights fp32 [D]; gate [gate_rows, D], its row gate_index[m]
     (int32 [rows]) for row m, or one gate row for all, or one per row."""
     if stream is not None:
-        with _on(stream):
+        with _on(stream, _device(y)):
             return norm_residual(y, x, w_pre, w_post, gate, gate_index, alpha, eps, h_out, n_out)
     return _torch.norm_residual(y, x, w_pre, w_post, gate, gate_index, alpha, eps, h_out, n_out)

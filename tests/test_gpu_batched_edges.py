@@ -78,3 +78,17 @@ def test_rope_append_of_few_small_heads(H, KVH, D, rotate):
     if KVH:
         R.assert_within(ck.flatten(0, 1)[slot], *turned(k), "k")
         assert torch.equal(cv.flatten(0, 1)[slot], v)
+
+
+def test_flags_that_have_no_truth_value():
+    """Their own error, before anything is launched."""
+    class Neither:
+        def __bool__(self):
+            raise ArithmeticError("neither")
+
+    pool = Pool([40], 16, 2, 64, BF16)
+    q = torch.zeros(1, 4, 64, device="cuda", dtype=BF16)
+    with pytest.raises(ArithmeticError):
+        voxq.paged_attention(q, pool.k, pool.v, pool.table, ints([0, 1]), ints([40]), 1, 40, causal=Neither())
+    with pytest.raises(ArithmeticError):
+        voxq.rope_append(q, q[:, :2], q[:, :2], voxq.rope_freqs(4, 64), ints([0]), ints([0], torch.int64), pool.k, pool.v, interleaved=Neither())

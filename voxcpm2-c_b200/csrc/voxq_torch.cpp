@@ -83,6 +83,11 @@ int as_i32(PyObject* o, const char* what) {
     need(v >= INT32_MIN && v <= INT32_MAX, what);
     return (int)v;
 }
+bool as_bool(PyObject* o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw Raised{};
+    return v != 0;
+}
 float as_float(PyObject* o) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) throw Raised{};
@@ -167,7 +172,7 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         d.heads = i32(H);
         d.kv_heads = i32(KVH);
         d.head_dim = i32(D);
-        d.interleaved = PyObject_IsTrue(a[9]);
+        d.interleaved = as_bool(a[9]);
         d.pages = i32(ck.size(0));
         d.page_size = i32(ck.size(1));
         d.in_dtype = code_of(q.scalar_type());
@@ -220,7 +225,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         d.total_q = i32(q.size(0));
         d.dtype = code_of(q.scalar_type());
         d.out_dtype = code_of(out.scalar_type());
-        d.causal = PyObject_IsTrue(a[8]);
+        d.causal = as_bool(a[8]);
         d.scale = as_float(a[9]);
         const size_t bytes = g.paged_workspace(&d);
         at::Tensor ws;

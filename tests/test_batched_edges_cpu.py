@@ -2,8 +2,10 @@
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 import subprocess
+import sys
 
 import pytest
 
@@ -90,3 +92,34 @@ def test_streams_of_another_gpu_are_refused():
             voxq.norm_residual(y, y, stream=Stream())
     with pytest.raises(ValueError):
         voxq.norm_residual(torch.zeros(2, 64), torch.zeros(2, 64), stream=Stream())
+
+
+def _build_module(tmp_path, monkeypatch):
+    spec = importlib.util.spec_from_file_location("voxq_build", os.path.join(REPO, "voxcpm2-c_b200", "build.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    (tmp_path / "voxq").mkdir()
+    monkeypatch.setattr(m, "HERE", str(tmp_path))
+    monkeypatch.setattr(m, "OBJ", str(tmp_path / "_build"))
+    ran = []
+
+    def compiled(cmd, **kw):
+        ran.append(cmd)
+        (tmp_path / "voxq" / "_torch.so").write_text("")
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+    monkeypatch.setattr(m.subprocess, "run", compiled)
+    return m, ran
+
+
+def test_the_library_builds_without_pytorch(tmp_path, monkeypatch):
+    m, ran = _build_module(tmp_path, monkeypatch)
+    monkeypatch.setitem(sys.modules, "torch", None)  # its import then fails
+    assert m.build_binding() is None and not ran
+
+
+def test_the_binding_is_rebuilt_for_another_torch(tmp_path, monkeypatch):
+    m, ran = _build_module(tmp_path, monkeypatch)
+    assert m.build_binding() and len(ran) == 1
+    assert m.build_binding() and len(ran) == 1
+    monkeypatch.setattr(torch, "__version__", "0.0.another")
+    assert m.build_binding() and len(ran) == 2

@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
-"""Builds libvoxq.so (all CUDA sources for sm_100a) next to this file, and the binding of the batched
-operators to torch tensors (csrc/voxq_torch.cpp) as voxq/_torch.so.
+"""Builds libvoxq.so (all CUDA sources for sm_100a) next to this file and, where PyTorch is installed, the binding of
+the batched operators to torch tensors (csrc/voxq_torch.cpp) as voxq/_torch.so.  A C user needs nvcc alone.
 
     python voxcpm2-c_b200/build.py [-j N] [--force]
 
@@ -72,13 +72,20 @@ def build(force: bool = False, jobs: int = 8, verbose: bool = False) -> str:
     return LIB
 
 
-def build_binding(force: bool = False) -> str:
-    """voxq/_torch.so: a CPython module against the installed torch's headers and libraries."""
+def build_binding(force: bool = False) -> str | None:
+    """voxq/_torch.so: a CPython module against the installed torch's headers and libraries; rebuilt when its source or
+    either of them changes.  Without PyTorch there is nothing to bind: returns None."""
     import sysconfig
-    import torch
+    try:
+        import torch
+    except ImportError:
+        sys.stderr.write("no PyTorch: voxq/_torch.so (the batched operators on torch tensors) is not built\n")
+        return None
     src, out = os.path.join(CSRC, "voxq_torch.cpp"), os.path.join(HERE, "voxq", "_torch.so")
     header = os.path.join(REPO, "include", "voxq.h")
-    if not force and os.path.exists(out) and os.path.getmtime(out) > max(os.path.getmtime(src), os.path.getmtime(header)):
+    stamp, made = os.path.join(OBJ, "_torch.stamp"), f"torch {torch.__version__} at {torch.__file__}, Python {sys.version}\n"
+    if not force and os.path.exists(out) and os.path.exists(stamp) and open(stamp).read() == made and \
+            os.path.getmtime(out) > max(os.path.getmtime(src), os.path.getmtime(header)):
         return out
     root = os.path.dirname(torch.__file__)
     lib, inc = os.path.join(root, "lib"), os.path.join(root, "include")
@@ -91,6 +98,9 @@ def build_binding(force: bool = False) -> str:
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError(f"g++ failed on {src}")
+    os.makedirs(OBJ, exist_ok=True)
+    with open(stamp, "w") as f:
+        f.write(made)
     return out
 
 

@@ -89,6 +89,8 @@ def matmul_nt(a, w, out=None) -> np.ndarray:
     N = w.shape[0]
     if out is None:
         out = np.zeros((M, N), dtype=np.float32)
+    elif out.dtype != np.float32 or out.shape != (M, N) or not out.flags.c_contiguous or not out.flags.writeable:
+        raise ValueError(f"out: a writeable, contiguous float32 array of {M} x {N} is needed")
     lib().oracle_matmul_nt(ap, wp, out.ctypes.data_as(C.POINTER(C.c_float)), M, N, K)
     return out
 

@@ -570,7 +570,8 @@ VOXQ_API VoxCPMError voxq_rope_append(const voxq_rope* d, void* stream);
  * In the 16-bit types the products take 16-bit operands with fp32
  * accumulation.  The softmax weights enter the second product with 16
  * significant bits or more when out is VOXQ_F32, and otherwise with at least as
- * many as out keeps (8 in bf16, 11 in fp16).  max_q and max_kv are upper bounds
+ * many as out keeps (8 in bf16, 11 in fp16).  Infinities and NaN count as in
+ * the formula: in the rows that see them and have a weight for them.  max_q and max_kv are upper bounds
  * of the sequences' new tokens and lengths (they choose the kernel and size
  * its grid; kv_len is clamped to max_kv).  16-byte rows; head_dim a multiple
  * of 8 up to 256; heads / kv_heads any whole number.

@@ -92,3 +92,79 @@ def test_flags_that_have_no_truth_value():
         voxq.paged_attention(q, pool.k, pool.v, pool.table, ints([0, 1]), ints([40]), 1, 40, causal=Neither())
     with pytest.raises(ArithmeticError):
         voxq.rope_append(q, q[:, :2], q[:, :2], voxq.rope_freqs(4, 64), ints([0]), ints([0], torch.int64), pool.k, pool.v, interleaved=Neither())
+
+
+def attention_by_the_formula(q, ck, cv, table, cu, kv_len, out_dtype):
+    """(result, bound) in float64, causal, each row over the keys that it sees and no others, so that what is not finite
+    is so by the formula."""
+    u = 0.0 if q.dtype is F32 else R.U[q.dtype]
+    uo = R.U[out_dtype or q.dtype]
+    q, ck, cv, table = R.f8(q), R.f8(ck), R.f8(cv), table.cpu().long()
+    D, page, G = q.shape[2], ck.shape[1], q.shape[1] // ck.shape[2]
+    out, bound = torch.zeros_like(q), torch.zeros_like(q)
+    for s, L in enumerate(kv_len.tolist()):
+        lo, hi = int(cu[s]), int(cu[s + 1])
+        pos = torch.arange(L)
+        at = table[s, pos // page] * page + pos % page
+        for i in range(hi - lo):
+            see = max(min(L - (hi - lo) + i + 1, L), 0)
+            if see == 0:
+                continue
+            for h in range(q.shape[1]):
+                k, v, x = ck.flatten(0, 1)[at[:see], h // G], cv.flatten(0, 1)[at[:see], h // G], q[lo + i, h]
+                sc = (k @ x) * D ** -0.5
+                p = torch.softmax(sc, 0)
+                fine = torch.nan_to_num(v, 0, 0, 0).abs()
+                out[lo + i, h] = (p[:, None] * v).sum(0)
+                delta = (torch.nan_to_num(k, 0, 0, 0).abs() @ x.abs()).amax() * D ** -0.5 * (D + 4) * R.E
+                bound[lo + i, h] = uo * out[lo + i, h].abs() + (2 * u + 4 * delta + (L + 8) * R.E) * (torch.nan_to_num(p)[:, None] * fine).sum(0)
+    return out, bound
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(F32, None), (F16, None), (F16, F32), (BF16, None), (BF16, F32)], ids=ids)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows,more", [(4, 0), (12, 0), (40, 60)], ids=["step", "few", "many"])
+def test_attention_that_meets_infinities_and_nan(rows, more, dim, dtype, out_dtype):
+    """Infinite and NaN keys and values, seen and not seen, give what the formula gives in every kernel: not finite where it
+    is not, and unharmed elsewhere."""
+    inf, nan = float("inf"), float("nan")
+    # sequence: 0, 1 values, 2 keys, 3 its last token, 4 fewer keys than rows, 5 a single key, 6 on unharmed
+    n = [rows] * 5 + [1] + [rows] * (1 + more)
+    lens = [200, 150, 130, rows + 40, rows - 2, 1] + [rows + 24] * (1 + more)
+    pool = Pool(lens, 16, 2, dim, dtype, seed=3)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q = torch.randn(sum(n), 8, dim, generator=g, device="cuda")
+    cu = starts(n)
+    q[cu[2]:cu[3], :, 5] = q[cu[2]:cu[3], :, 5].abs() + 0.1
+    q[cu[2] + 1, :, 5] *= -1
+    q[cu[1], 3, 7] = inf
+    q[cu[5], :, 2] = 1e-37 if dtype is F32 else 0
+    q = q.to(dtype)
+    top = torch.finfo(dtype).max
+
+    def put(cache, s, j, kvh, dims, value):
+        cache[int(pool.table[s, j // 16]), j % 16, kvh, dims] = value
+    put(pool.v, 0, 3, 0, 9, inf)
+    put(pool.v, 0, 100, 0, 10, -inf)
+    put(pool.v, 0, 101, 0, 11, nan)
+    put(pool.v, 0, 7, 0, 12, inf)
+    put(pool.v, 0, 150, 0, 12, -inf)
+    put(pool.v, 1, lens[1] - 2, 1, slice(0, 40), inf)   # not seen by the first rows
+    put(pool.k, 2, 20, 0, 5, -inf)                      # weight 0; a NaN for the row whose query is negative there
+    put(pool.k, 2, 90, 0, 5, -inf)
+    put(pool.k, 3, lens[3] - 1, 0, slice(None), nan)    # seen by the last row alone
+    put(pool.v, 3, lens[3] - 1, 1, slice(None), nan)
+    put(pool.v, 4, 0, 0, slice(None), nan)
+    put(pool.v, 4, 1, 1, 3, -inf)
+    put(pool.v, 5, 0, 0, slice(0, 8), top)
+    put(pool.k, 5, 0, 1, 2, top)
+    cu, kv = ints(cu), ints(lens)
+    o = voxq.paged_attention(q, pool.k, pool.v, pool.table, cu, kv, max(n), max(lens), out_dtype=out_dtype)
+    some = 8
+    ref, bound = attention_by_the_formula(q[:int(cu[some - 1])], pool.k, pool.v, pool.table, cu[:some], kv[:some - 1], out_dtype)
+    y = R.f8(o)[:ref.shape[0]]
+    assert torch.equal(torch.isnan(y), torch.isnan(ref)), "NaN in other places than the formula's"
+    fine = torch.isfinite(ref)
+    assert torch.equal(y[~fine & ~torch.isnan(ref)], ref[~fine & ~torch.isnan(ref)]), "infinities in other places than the formula's"
+    R.assert_within(torch.where(fine, y, 0.0), torch.where(fine, ref, 0.0), torch.where(fine, bound, 0.0) + R.TINY[out_dtype or dtype])
+    assert torch.isfinite(o[int(cu[6]):]).all() and int(voxq.lib().voxq_device_error(1)) == 0

@@ -167,13 +167,22 @@ __global__ void __launch_bounds__(kMmaThreads) paged_mma_kernel(const __grid_con
         }
     }
     // A row's result goes to out, or, when its keys fill more than one split, to this split's record.
+    bool again[2] = {false, false}, weights[2];
 #pragma unroll
     for (int e = 0; e < 2; e++) {
         const int r = row[e];
         if (r >= n * G) continue;
         const int tok = first + r / G, h = kh * G + r % G, seen = visible(p, len, n, r / G);
+        float chk = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NB; j++) chk = fmaf(o[j][2 * e], 0.0f, fmaf(o[j][2 * e + 1], 0.0f, chk));
+        again[e] = not_finite<T>(chk, l[e]);
+        weights[e] = l[e] == l[e];
         if (seen <= p.split_len) {
-            if (blockIdx.z > 0) continue;
+            if (blockIdx.z > 0) {
+                again[e] = false;
+                continue;
+            }
             const float inv = seen > 0 ? 1.0f / l[e] : 0.0f;
             const int64_t at = tok * d.o_stride + h * d.o_head_stride;
 #pragma unroll
@@ -186,7 +195,22 @@ __global__ void __launch_bounds__(kMmaThreads) paged_mma_kernel(const __grid_con
             for (int j = 0; j < NB; j++)
                 if (j * 8 < d.head_dim)
                     *reinterpret_cast<float2*>(p.acc + rec * d.head_dim + j * 8 + 2 * t) = make_float2(o[j][2 * e], o[j][2 * e + 1]);
+        } else {
+            again[e] = false;
         }
+    }
+    uint32_t rows_again = 0;  // bit 8 e + g: a lane of row g + 8 e found something; bit 16 more: its weights are not finite
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+        if (again[e]) rows_again |= (weights[e] ? 1u : 0x10001u) << (8 * e + g);
+    rows_again = __reduce_or_sync(0xffffffffu, rows_again);
+    if (rows_again == 0) return;
+    __syncwarp();  // what this warp wrote is read
+    RowsAgain<T> found(k_beg);
+    for (int i = 0; i < 16; i++) {
+        const int r = r0 + wm * 16 + i, seen = visible(p, len, n, r / G);
+        const int64_t rec = ((int64_t)(first + r / G) * d.heads + kh * G + r % G) * p.splits + blockIdx.z;
+        if (rows_again >> i & 1) found.row(p, s, first, r, kh, k_beg, min(seen, k_stop), seen <= p.split_len ? -1 : rec, !(rows_again >> (16 + i) & 1));
     }
 }
 

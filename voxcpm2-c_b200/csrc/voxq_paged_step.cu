@@ -288,6 +288,8 @@ __global__ void __launch_bounds__(kStepThreads, StepShape<T, HD>::per_sm) paged_
         }
         __syncthreads();
         const int r = threadIdx.x >> 3, row = r0 + r;  // 8 threads a row
+        const bool all = a == 0 && b == q.tiles;
+        uint32_t rows_again = 0;
         if (r < rows && ok) {
             float mm = -INFINITY, ll = 0.0f, f[W];
 #pragma unroll
@@ -298,11 +300,11 @@ __global__ void __launch_bounds__(kStepThreads, StepShape<T, HD>::per_sm) paged_
                 ll = fmaf(wml[w][r].y, f[w], ll);
             }
             // all of the row's keys: to out; else the block's first piece (0) or its last (1)
-            const bool all = a == 0 && b == q.tiles;
             const float inv = !all ? 1.0f : visible(p, q.len, q.n, row / G) > 0 ? 1.0f / ll : 0.0f;
             const int64_t rec = (blockIdx.x * 2 + (again ? 1 : 0)) * 16 + r;
             const int64_t at = (q.first + row / G) * d.o_stride + (kh * G + row % G) * d.o_head_stride;
             if (!all && (threadIdx.x & 7) == 0) p.ml[rec] = make_float2(mm, ll);
+            float chk = 0.0f;
             for (int x = (threadIdx.x & 7) * 2; x < d.head_dim; x += 16) {
                 float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -311,9 +313,20 @@ __global__ void __launch_bounds__(kStepThreads, StepShape<T, HD>::per_sm) paged_
                     v.x = fmaf(y.x, f[w], v.x);
                     v.y = fmaf(y.y, f[w], v.y);
                 }
+                chk = fmaf(v.x, 0.0f, fmaf(v.y, 0.0f, chk));
                 if (all) store_pair<T>(p, at + x, v.x * inv, v.y * inv);
                 else *reinterpret_cast<float2*>(p.acc + rec * d.head_dim + x) = v;
             }
+            if (not_finite<T>(chk, ll)) rows_again = (ll == ll ? 1u : 0x10001u) << r;
+        }
+        rows_again = __reduce_or_sync(0xffffffffu, rows_again);
+        if (rows_again) {  // (of this warp's four)
+            __syncwarp();  // what this warp wrote is read
+            RowsAgain<T> found(a * KT);
+            for (int i = warp * 4; i < warp * 4 + 4; i++)
+                if (rows_again >> i & 1)
+                    found.row(p, it.s, q.first, r0 + i, kh, a * KT, min(visible(p, q.len, q.n, (r0 + i) / G), k_stop),
+                              all ? -1 : (int64_t)(blockIdx.x * 2 + (again ? 1 : 0)) * 16 + i, !(rows_again >> (16 + i) & 1));
         }
         __syncthreads();  // the joined outputs and the queries are read
     }

@@ -9,7 +9,7 @@
 namespace voxq {
 
 constexpr int kTcTile = 128;                 // rows of a query tile, keys of a key tile
-constexpr int kTcThreads = 384;              // two softmax warpgroups; loader, MMA and unit warps, one idle
+constexpr int kTcThreads = 384;              // two softmax warpgroups; loader, MMA and unit warps, one for rows to put right
 constexpr int kTcRegsSoftmax = 208, kTcRegsOther = 80;  // 256 * 208 + 128 * 80 <= the 384 * 168 of the launch
 template <int HD>
 constexpr int kTcTiles = HD > 128 ? 1 : 2;   // query tiles of a unit: tensor memory holds the output of 256 columns once
@@ -184,6 +184,8 @@ __device__ __forceinline__ bool next_block(const uint4* answer, int& x, int& y, 
 //                   zeroes the values past a unit's last key
 //   warp 9          issues S = Q K^T and O += P V
 //   warp 10         finds the units: this block's own, then those of blocks that have not started
+//   warp 11         puts rows right that met something not finite, behind their output: on the softmax warps the same code,
+//                   though never run, cost their loop the registers for a tenth of the prompts' time
 // Tensor memory: S0, S1 (128 columns each, P over their first 64, its low part over the rest), O0, O1.  The tensor pipe runs one thread's MMAs in
 // order, so the S of the next key tile may follow the PV that still reads P, and a thread that has seen S complete
 // knows that every earlier PV is complete too: it may rescale O without a barrier of its own.  Rescaling is rare: sums
@@ -209,14 +211,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     constexpr int TILE = kTcTileBytes<HD>, ST = kTcStages<HD>, TW = kTcTiles<HD>, ROWS = TW * kTcTile;
     static_assert(ST < 2 * kTcTails, "as many mended ends as the ring can hold");
     extern __shared__ uint8_t tc_raw[];
-    __shared__ uint64_t bar[2 * ST + 2 * kTcItems + 10 + kTcTails];
+    __shared__ uint64_t bar[2 * ST + 3 * kTcItems + 10 + kTcTails];
     __shared__ uint4 answer;
     __shared__ TcItem items[kTcItems];
+    __shared__ uint32_t again[kTcItems][8];  // by softmax warp: rows of a unit whose sums are not finite
     __shared__ uint32_t tmem_slot;
     uint64_t *full = bar, *empty = full + ST;                                // ring
     uint64_t *s_full = empty + ST, *p_full = s_full + 2;  // per query tile
     uint64_t *o_done = p_full + 2, *q_full = o_done + 2;
-    uint64_t *item_full = q_full + 2, *item_empty = item_full + kTcItems, *tail = item_empty + kTcItems, *asked = tail + kTcTails, *begun = asked + 1;
+    uint64_t *item_full = q_full + 2, *item_empty = item_full + kTcItems, *tail = item_empty + kTcItems, *asked = tail + kTcTails, *begun = asked + 1, *written = begun + 1;
     const voxq_paged_attn& d = p.d;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, G = p.group;
     const uint32_t qsm = (smem_u32(tc_raw) + 1023) & ~1023u, ring = qsm + TW * TILE;
@@ -235,7 +238,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         for (int i = 0; i < kTcTails; i++) mbar_init(tail + i, 1);
         for (int i = 0; i < kTcItems; i++) {
             mbar_init(item_full + i, 1);
-            mbar_init(item_empty + i, 10);  // every warp that works on units
+            mbar_init(item_empty + i, 11);  // every warp that works on units
+            mbar_init(written + i, 8);
         }
         mbar_init(asked, 1);
         mbar_init(begun, 1);
@@ -268,7 +272,226 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         return ok;
     };
 
-    if (warp >= 8) {
+    if (warp < 8) {
+        // ---------------- softmax and output: one row a thread ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTcRegsSoftmax));
+        const int t = warp >> 2, lr = threadIdx.x & 127;
+        const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * kTcTile, to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 256 + t * HD;
+        // The warp's 32 rows of queries, HD / 8 lanes a row so that every load covers whole lines, and their place in
+        // shared memory: 16-byte chunk j of a 128-byte row at chunk j ^ (row & 7).
+        constexpr int CPR = HD / 8, STEP = 32 / CPR;  // chunks of a row, rows of an access
+        const int cj = lane % CPR, crow = lane / CPR;
+        auto place = [&](int row, int j) {
+            return qsm + t * TILE + (j / 8) * kTcHalf + ((warp & 3) * 32 + row) * 128 + (((j % 8) ^ (row & 7)) << 4);
+        };
+        auto load_q = [&](const TcItem& u) {
+            const int row0 = t * kTcTile + (warp & 3) * 32 + crow, r = u.r0 + row0;
+            int tok = r / G, h = r % G;
+            constexpr int BATCH = CPR < 16 ? CPR : 16;
+            uint4 v[BATCH];
+#pragma unroll
+            for (int i0 = 0; i0 < CPR; i0 += BATCH) {
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) {
+                    v[i] = make_uint4(0, 0, 0, 0);
+                    if (row0 + (i0 + i) * STEP < u.rows && cj * 8 < d.head_dim)
+                        v[i] = *reinterpret_cast<const uint4*>((const T*)d.q + (u.first + tok) * d.q_stride + (u.kh * G + h) * d.q_head_stride + cj * 8);
+                    for (h += STEP; h >= G; h -= G) tok++;
+                }
+#pragma unroll
+                for (int i = 0; i < BATCH; i++) sts128(place(crow + (i0 + i) * STEP, cj), v[i]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full + t);
+        };
+        // (a unit's fields are read from shared memory where they are needed: the loop over its keys wants the registers)
+        bool ok = unit_ready(0);
+        uint32_t step = 0, unit = 0;
+        if (ok && items[0].has(t) && items[0].tiles() > 0) load_q(items[0]);
+        for (int k = 0; ok && items[k % kTcItems].rows > 0; k++) {
+            const TcItem& it = items[k % kTcItems];
+            const int tiles = it.has(t) ? it.tiles() : 0;
+            const bool mine = t * kTcTile + lr < it.rows;
+            const int vis = mine ? min(visible(p, it.len, it.n, (it.r0 + t * kTcTile + lr) / G), it.k_stop) : 0;
+            // keys that every row of the tile sees need no mask
+            const int all_see = min(visible(p, it.len, it.n, (it.r0 + t * kTcTile) / G), it.k_stop);
+            int t0 = it.k_beg;
+            float m = -INFINITY, l = 0.0f;  // m in base-2 units
+            for (int i = 0; i < tiles; i++, t0 += kTcTile) {
+                ok = warp_wait(s_full + t, step++ & 1, VOXQ_DEVERR_WAIT_MMA, p.err);
+                if (!ok) break;
+                tc_after();
+                uint32_t sv[kTcTile], low[LOW ? kTcTile / 2 : 1];
+                uint64_t sum[2];
+                // The weights are taken relative to the maximum so far, while this tile's maximum is found beside them:
+                // only if a row has outgrown its own by 2^8 are sums rescaled and the tile's weights computed again.
+                while (true) {
+#pragma unroll
+                    for (int c = 0; c < kTcTile; c += 32) tm_ld32(ts + c, sv + c);
+                    tm_wait_ld();
+                    if (t0 + kTcTile > all_see) {
+#pragma unroll
+                        for (int c = 0; c < kTcTile; c++)
+                            if (t0 + c >= vis) sv[c] = __float_as_uint(-INFINITY);
+                    }
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    auto row_max = [&](int c) {  // of 16 scores
+#pragma unroll
+                        for (int e = 0; e < 16; e += 8)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) mx[j] = fmaxf(fmaxf(mx[j], __uint_as_float(sv[c + e + j])), __uint_as_float(sv[c + e + j + 4]));
+                    };
+                    auto top = [&] { return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale2; };
+                    if (i == 0) {
+#pragma unroll
+                        for (int c = 0; c < kTcTile; c += 16) row_max(c);
+                        m = top();
+                    }
+                    const float neg = m == -INFINITY ? 0.0f : -m;  // no key so far: every weight is ex2(-inf) = 0
+                    const uint64_t sc2 = pk(p.scale2, p.scale2), ng2 = pk(neg, neg);
+                    sum[0] = sum[1] = pk(0.0f, 0.0f);
+                    // One pair of exponentials after the other, the scaling of a later pair and the sums and rounding of an
+                    // earlier one between them: a lone warp keeps its special-function unit busy only if nothing else
+                    // is issued in a bunch.
+                    constexpr int AHEAD = 3, BEHIND = 3;
+                    uint64_t x[kTcTile / 2];
+                    float y[kTcTile];
+                    auto scaled = [&](int c) { x[c] = fma2v(pk(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1])), sc2, ng2); };
+#pragma unroll
+                    for (int c = 0; c < AHEAD; c++) scaled(c);
+#pragma unroll
+                    for (int c = 0; c < kTcTile / 2 + BEHIND; c++) {
+                        if (c < kTcTile / 2) {
+                            upk(x[c], y[2 * c], y[2 * c + 1]);
+                            y[2 * c] = ex2v(y[2 * c]);
+                        }
+                        if (c + AHEAD < kTcTile / 2) scaled(c + AHEAD);
+                        if (c < kTcTile / 2) {
+                            mx[c & 3] = max3v(mx[c & 3], __uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1]));
+                            y[2 * c + 1] = ex2v(y[2 * c + 1]);
+                        }
+                        if (c >= BEHIND) {
+                            const int o = c - BEHIND;
+                            sum[o & 1] = add2v(sum[o & 1], pk(y[2 * o], y[2 * o + 1]));
+                            sv[o] = pack2v<T>(y[2 * o], y[2 * o + 1]);  // (over scores that are done with)
+                            if (LOW) low[o] = rest2v<T>(sv[o], y[2 * o], y[2 * o + 1]);
+                        }
+                    }
+                    const float mt = top();
+                    const bool grow = mt > m + kTcSlack;
+                    if (!__any_sync(0xffffffffu, grow)) break;
+                    const float f = grow ? ex2(m - mt) : 1.0f;
+                    if (grow) m = mt;
+                    l *= f;
+#pragma unroll
+                    for (int c = 0; c < HD; c += 32) {  // (i > 0: the first tile's weights are relative to its own maximum)
+                        uint32_t o[32];
+                        tm_ld32(to + c, o);
+                        tm_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tm_st32(to + c, o);
+                    }
+                }
+                tm_st32(ts, sv);
+                tm_st32(ts + 32, sv + 32);
+                if (LOW) {
+                    tm_st32(ts + 64, low);
+                    tm_st32(ts + 96, low + 32);
+                }
+                float a, b, e, f;
+                upk(sum[0], a, b);
+                upk(sum[1], e, f);
+                l += (a + b) + (e + f);
+                tm_wait_st();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + t);
+            }
+            // The next unit's queries start their way (into L2) while the last product runs.  Their buffer is free (this
+            // unit's last scores are complete): it first takes the output, so that rows leave in whole lines, then them.
+            ok = ok && unit_ready(k + 1);
+            const TcItem& next = items[(k + 1) % kTcItems];
+            const bool more = ok && next.has(t) && next.tiles() > 0;
+            if (more && t * kTcTile + lr < next.rows) {
+                const int r = next.r0 + t * kTcTile + lr;
+                const T* src = (const T*)d.q + (next.first + r / G) * d.q_stride + (next.kh * G + r % G) * d.q_head_stride;
+#pragma unroll
+                for (int c = 0; c < HD; c += 64)
+                    if (c < d.head_dim) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + c));
+            }
+            if (ok && tiles > 0) {
+                ok = warp_wait(o_done + t, unit++ & 1, VOXQ_DEVERR_WAIT_MMA, p.err);
+                tc_after();
+            }
+            uint32_t rows_again = 0;
+            if (it.has(t)) {
+                const int r = it.r0 + t * kTcTile + lr, tok = r / G, h = it.kh * G + r % G;
+                const int seen = mine ? visible(p, it.len, it.n, tok) : 0;
+                const bool whole = seen <= p.split_len;
+                // a row with more keys than a split holds leaves a record, one with fewer is split 0's
+                const bool put = ok && mine && (whole ? it.z == 0 : it.k_beg < seen);
+                const float inv = !whole ? 1.0f : seen > 0 ? 1.0f / l : 0.0f;
+                const int64_t rec = ((int64_t)(it.first + tok) * d.heads + h) * p.splits + it.z;
+                if (put && !whole) p.ml[rec] = make_float2(m, l);
+                const int64_t dst = whole ? (it.first + tok) * d.o_stride + h * d.o_head_stride : rec * d.head_dim;
+                const int kind = !put ? 0 : whole ? 1 : 2;
+                // 16-bit rows of the output at once, fp32 ones (records, or an fp32 output) in two halves of the head
+                const bool fast = d.out_dtype != VOXQ_F32 && __all_sync(0xffffffffu, kind < 2);
+                float chk[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+                for (int part = 0; part < (fast ? 1 : 2); part++) {
+#pragma unroll 1
+                    for (int c = 0; c < (fast ? HD : HD / 2); c += 32) {
+                        uint32_t o[32];
+                        if (tiles > 0) {
+                            tm_ld32(to + part * (HD / 2) + c, o);
+                            tm_wait_ld();
+                        }
+                        if (seen > 0 && tiles > 0)
+#pragma unroll
+                            for (int e = 0; e < 32; e++) chk[e & 3] = fmaf(__uint_as_float(o[e]), 0.0f, chk[e & 3]);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = seen > 0 ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
+                        if (fast) {
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = pack2<T>(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+                        }
+                        const int chunk = fast ? c / 8 : c / 4;
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            if (e < 4 || !fast)
+                                sts128(place(lane, chunk + e), make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
+                    }
+                    __syncwarp();
+#pragma unroll 4
+                    for (int i = 0; i < CPR; i++) {
+                        const int row = crow + i * STEP, what = __shfl_sync(0xffffffffu, kind, row);
+                        const int64_t at = __shfl_sync(0xffffffffu, dst, row);
+                        const uint4 v = lds128(place(row, cj));
+                        if (what == 0 || part * (HD / 2) + cj * (fast ? 8 : 4) >= d.head_dim) continue;
+                        if (fast) {
+                            *reinterpret_cast<uint4*>((T*)d.out + at + cj * 8) = v;
+                        } else {
+                            const int64_t x = at + part * (HD / 2) + cj * 4;
+                            if (what == 2) *reinterpret_cast<uint4*>(p.acc + x) = v;
+                            else if (d.out_dtype == VOXQ_F32) *reinterpret_cast<uint4*>((float*)d.out + x) = v;
+                            else *reinterpret_cast<uint2*>((T*)d.out + x) = make_uint2(pack2<T>(__uint_as_float(v.x), __uint_as_float(v.y)), pack2<T>(__uint_as_float(v.z), __uint_as_float(v.w)));
+                        }
+                    }
+                    __syncwarp();
+                }
+                rows_again = __ballot_sync(0xffffffffu, put && not_finite<T>((chk[0] + chk[1]) + (chk[2] + chk[3]), l));
+            }
+            if (lane == 0) again[k % kTcItems][warp] = rows_again;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(written + k % kTcItems);
+            if (more) load_q(next);
+            tc_before();  // the output is read before the next unit's first product may overwrite it (p_full)
+            done(k);
+        }
+    } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTcRegsOther));
         if (warp == 8) {
             // ---------------- loader: K0, V0, K1, V1, ... of every unit ----------------
@@ -524,216 +747,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             }
             it.rows = 0;
             if (ok) put(it);
-        }
-    } else {
-        // ---------------- softmax and output: one row a thread ----------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTcRegsSoftmax));
-        const int t = warp >> 2, lr = threadIdx.x & 127;
-        const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * kTcTile, to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 256 + t * HD;
-        // The warp's 32 rows of queries, HD / 8 lanes a row so that every load covers whole lines, and their place in
-        // shared memory: 16-byte chunk j of a 128-byte row at chunk j ^ (row & 7).
-        constexpr int CPR = HD / 8, STEP = 32 / CPR;  // chunks of a row, rows of an access
-        const int cj = lane % CPR, crow = lane / CPR;
-        auto place = [&](int row, int j) {
-            return qsm + t * TILE + (j / 8) * kTcHalf + ((warp & 3) * 32 + row) * 128 + (((j % 8) ^ (row & 7)) << 4);
-        };
-        auto load_q = [&](const TcItem& u) {
-            const int row0 = t * kTcTile + (warp & 3) * 32 + crow, r = u.r0 + row0;
-            int tok = r / G, h = r % G;
-            constexpr int BATCH = CPR < 16 ? CPR : 16;
-            uint4 v[BATCH];
-#pragma unroll
-            for (int i0 = 0; i0 < CPR; i0 += BATCH) {
-#pragma unroll
-                for (int i = 0; i < BATCH; i++) {
-                    v[i] = make_uint4(0, 0, 0, 0);
-                    if (row0 + (i0 + i) * STEP < u.rows && cj * 8 < d.head_dim)
-                        v[i] = *reinterpret_cast<const uint4*>((const T*)d.q + (u.first + tok) * d.q_stride + (u.kh * G + h) * d.q_head_stride + cj * 8);
-                    for (h += STEP; h >= G; h -= G) tok++;
-                }
-#pragma unroll
-                for (int i = 0; i < BATCH; i++) sts128(place(crow + (i0 + i) * STEP, cj), v[i]);
+        } else {
+            // ---------------- rows to put right: none, as a rule ----------------
+            // (the kernel's last code: between the others' it took 10 us more from cold caches)
+            for (int k = 0; unit_ready(k) && items[k % kTcItems].rows > 0; k++) {
+                const TcItem& it = items[k % kTcItems];
+                if (!__all_sync(0xffffffffu, mbar_wait_bounded(written + k % kTcItems, (k / kTcItems) & 1, VOXQ_DEVERR_WAIT_FULL, p.err, kTcLong))) break;
+                RowsAgain<T> found(it.k_beg);
+                for (int w = 0; w < 8; w++)
+                    for (uint32_t rows = again[k % kTcItems][w]; rows; rows &= rows - 1) {
+                        const int r = it.r0 + w * 32 + __ffs(rows) - 1, seen = visible(p, it.len, it.n, r / G);
+                        const int64_t rec = ((int64_t)(it.first + r / G) * d.heads + it.kh * G + r % G) * p.splits + it.z;
+                        found.row(p, it.table, it.first, r, it.kh, it.k_beg, min(seen, it.k_stop), seen <= p.split_len ? -1 : rec, true);
+                    }
+                done(k);
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full + t);
-        };
-        // (a unit's fields are read from shared memory where they are needed: the loop over its keys wants the registers)
-        bool ok = unit_ready(0);
-        uint32_t step = 0, unit = 0;
-        if (ok && items[0].has(t) && items[0].tiles() > 0) load_q(items[0]);
-        for (int k = 0; ok && items[k % kTcItems].rows > 0; k++) {
-            const TcItem& it = items[k % kTcItems];
-            const int tiles = it.has(t) ? it.tiles() : 0;
-            const bool mine = t * kTcTile + lr < it.rows;
-            const int vis = mine ? min(visible(p, it.len, it.n, (it.r0 + t * kTcTile + lr) / G), it.k_stop) : 0;
-            // keys that every row of the tile sees need no mask
-            const int all_see = min(visible(p, it.len, it.n, (it.r0 + t * kTcTile) / G), it.k_stop);
-            int t0 = it.k_beg;
-            float m = -INFINITY, l = 0.0f;  // m in base-2 units
-            for (int i = 0; i < tiles; i++, t0 += kTcTile) {
-                ok = warp_wait(s_full + t, step++ & 1, VOXQ_DEVERR_WAIT_MMA, p.err);
-                if (!ok) break;
-                tc_after();
-                uint32_t sv[kTcTile], low[LOW ? kTcTile / 2 : 1];
-                uint64_t sum[2];
-                // The weights are taken relative to the maximum so far, while this tile's maximum is found beside them:
-                // only if a row has outgrown its own by 2^8 are sums rescaled and the tile's weights computed again.
-                while (true) {
-#pragma unroll
-                    for (int c = 0; c < kTcTile; c += 32) tm_ld32(ts + c, sv + c);
-                    tm_wait_ld();
-                    if (t0 + kTcTile > all_see) {
-#pragma unroll
-                        for (int c = 0; c < kTcTile; c++)
-                            if (t0 + c >= vis) sv[c] = __float_as_uint(-INFINITY);
-                    }
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    auto row_max = [&](int c) {  // of 16 scores
-#pragma unroll
-                        for (int e = 0; e < 16; e += 8)
-#pragma unroll
-                            for (int j = 0; j < 4; j++) mx[j] = fmaxf(fmaxf(mx[j], __uint_as_float(sv[c + e + j])), __uint_as_float(sv[c + e + j + 4]));
-                    };
-                    auto top = [&] { return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale2; };
-                    if (i == 0) {
-#pragma unroll
-                        for (int c = 0; c < kTcTile; c += 16) row_max(c);
-                        m = top();
-                    }
-                    const float neg = m == -INFINITY ? 0.0f : -m;  // no key so far: every weight is ex2(-inf) = 0
-                    const uint64_t sc2 = pk(p.scale2, p.scale2), ng2 = pk(neg, neg);
-                    sum[0] = sum[1] = pk(0.0f, 0.0f);
-                    // One pair of exponentials after the other, the scaling of a later pair and the sums and rounding of an
-                    // earlier one between them: a lone warp keeps its special-function unit busy only if nothing else
-                    // is issued in a bunch.
-                    constexpr int AHEAD = 3, BEHIND = 3;
-                    uint64_t x[kTcTile / 2];
-                    float y[kTcTile];
-                    auto scaled = [&](int c) { x[c] = fma2v(pk(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1])), sc2, ng2); };
-#pragma unroll
-                    for (int c = 0; c < AHEAD; c++) scaled(c);
-#pragma unroll
-                    for (int c = 0; c < kTcTile / 2 + BEHIND; c++) {
-                        if (c < kTcTile / 2) {
-                            upk(x[c], y[2 * c], y[2 * c + 1]);
-                            y[2 * c] = ex2v(y[2 * c]);
-                        }
-                        if (c + AHEAD < kTcTile / 2) scaled(c + AHEAD);
-                        if (c < kTcTile / 2) {
-                            mx[c & 3] = max3v(mx[c & 3], __uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1]));
-                            y[2 * c + 1] = ex2v(y[2 * c + 1]);
-                        }
-                        if (c >= BEHIND) {
-                            const int o = c - BEHIND;
-                            sum[o & 1] = add2v(sum[o & 1], pk(y[2 * o], y[2 * o + 1]));
-                            sv[o] = pack2v<T>(y[2 * o], y[2 * o + 1]);  // (over scores that are done with)
-                            if (LOW) low[o] = rest2v<T>(sv[o], y[2 * o], y[2 * o + 1]);
-                        }
-                    }
-                    const float mt = top();
-                    const bool grow = mt > m + kTcSlack;
-                    if (!__any_sync(0xffffffffu, grow)) break;
-                    const float f = grow ? ex2(m - mt) : 1.0f;
-                    if (grow) m = mt;
-                    l *= f;
-#pragma unroll
-                    for (int c = 0; c < HD; c += 32) {  // (i > 0: the first tile's weights are relative to its own maximum)
-                        uint32_t o[32];
-                        tm_ld32(to + c, o);
-                        tm_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tm_st32(to + c, o);
-                    }
-                }
-                tm_st32(ts, sv);
-                tm_st32(ts + 32, sv + 32);
-                if (LOW) {
-                    tm_st32(ts + 64, low);
-                    tm_st32(ts + 96, low + 32);
-                }
-                float a, b, e, f;
-                upk(sum[0], a, b);
-                upk(sum[1], e, f);
-                l += (a + b) + (e + f);
-                tm_wait_st();
-                tc_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + t);
-            }
-            // The next unit's queries start their way (into L2) while the last product runs.  Their buffer is free (this
-            // unit's last scores are complete): it first takes the output, so that rows leave in whole lines, then them.
-            ok = ok && unit_ready(k + 1);
-            const TcItem& next = items[(k + 1) % kTcItems];
-            const bool more = ok && next.has(t) && next.tiles() > 0;
-            if (more && t * kTcTile + lr < next.rows) {
-                const int r = next.r0 + t * kTcTile + lr;
-                const T* src = (const T*)d.q + (next.first + r / G) * d.q_stride + (next.kh * G + r % G) * d.q_head_stride;
-#pragma unroll
-                for (int c = 0; c < HD; c += 64)
-                    if (c < d.head_dim) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + c));
-            }
-            if (ok && tiles > 0) {
-                ok = warp_wait(o_done + t, unit++ & 1, VOXQ_DEVERR_WAIT_MMA, p.err);
-                tc_after();
-            }
-            if (it.has(t)) {
-                const int r = it.r0 + t * kTcTile + lr, tok = r / G, h = it.kh * G + r % G;
-                const int seen = mine ? visible(p, it.len, it.n, tok) : 0;
-                const bool whole = seen <= p.split_len;
-                // a row with more keys than a split holds leaves a record, one with fewer is split 0's
-                const bool put = ok && mine && (whole ? it.z == 0 : it.k_beg < seen);
-                const float inv = !whole ? 1.0f : seen > 0 ? 1.0f / l : 0.0f;
-                const int64_t rec = ((int64_t)(it.first + tok) * d.heads + h) * p.splits + it.z;
-                if (put && !whole) p.ml[rec] = make_float2(m, l);
-                const int64_t dst = whole ? (it.first + tok) * d.o_stride + h * d.o_head_stride : rec * d.head_dim;
-                const int kind = !put ? 0 : whole ? 1 : 2;
-                // 16-bit rows of the output at once, fp32 ones (records, or an fp32 output) in two halves of the head
-                const bool fast = d.out_dtype != VOXQ_F32 && __all_sync(0xffffffffu, kind < 2);
-#pragma unroll 1
-                for (int part = 0; part < (fast ? 1 : 2); part++) {
-#pragma unroll 1
-                    for (int c = 0; c < (fast ? HD : HD / 2); c += 32) {
-                        uint32_t o[32];
-                        if (tiles > 0) {
-                            tm_ld32(to + part * (HD / 2) + c, o);
-                            tm_wait_ld();
-                        }
-#pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = seen > 0 ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
-                        if (fast) {
-#pragma unroll
-                            for (int e = 0; e < 16; e++) o[e] = pack2<T>(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
-                        }
-                        const int chunk = fast ? c / 8 : c / 4;
-#pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            if (e < 4 || !fast)
-                                sts128(place(lane, chunk + e), make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]));
-                    }
-                    __syncwarp();
-#pragma unroll 4
-                    for (int i = 0; i < CPR; i++) {
-                        const int row = crow + i * STEP, what = __shfl_sync(0xffffffffu, kind, row);
-                        const int64_t at = __shfl_sync(0xffffffffu, dst, row);
-                        const uint4 v = lds128(place(row, cj));
-                        if (what == 0 || part * (HD / 2) + cj * (fast ? 8 : 4) >= d.head_dim) continue;
-                        if (fast) {
-                            *reinterpret_cast<uint4*>((T*)d.out + at + cj * 8) = v;
-                        } else {
-                            const int64_t x = at + part * (HD / 2) + cj * 4;
-                            if (what == 2) *reinterpret_cast<uint4*>(p.acc + x) = v;
-                            else if (d.out_dtype == VOXQ_F32) *reinterpret_cast<uint4*>((float*)d.out + x) = v;
-                            else *reinterpret_cast<uint2*>((T*)d.out + x) = make_uint2(pack2<T>(__uint_as_float(v.x), __uint_as_float(v.y)), pack2<T>(__uint_as_float(v.z), __uint_as_float(v.w)));
-                        }
-                    }
-                    __syncwarp();
-                }
-            }
-            if (more) load_q(next);
-            tc_before();  // the output is read before the next unit's first product may overwrite it (p_full)
-            done(k);
         }
     }
     tc_before();

@@ -168,3 +168,25 @@ def test_attention_that_meets_infinities_and_nan(rows, more, dim, dtype, out_dty
     assert torch.equal(y[~fine & ~torch.isnan(ref)], ref[~fine & ~torch.isnan(ref)]), "infinities in other places than the formula's"
     R.assert_within(torch.where(fine, y, 0.0), torch.where(fine, ref, 0.0), torch.where(fine, bound, 0.0) + R.TINY[out_dtype or dtype])
     assert torch.isfinite(o[int(cu[6]):]).all() and int(voxq.lib().voxq_device_error(1)) == 0
+
+
+def test_units_of_work_that_last_long():
+    """Every unit of 32 tokens ends in one with a NaN that the others do not see, so that its rows are taken again one by one:
+    units of some 0.1 s, several a block, whose waits must not give up."""
+    n, dim = [4100, 4096, 3000], 128
+    pool = Pool(n, 16, 2, dim, BF16, seed=8)
+    q = torch.randn(sum(n), 16, dim, generator=torch.Generator(device="cuda").manual_seed(8), device="cuda").to(BF16)
+    args = (pool.table, ints(starts(n)), ints(n), max(n), max(n))
+    clean = voxq.paged_attention(q, pool.k, pool.v, *args)
+    want = torch.zeros(sum(n), dim, dtype=torch.bool)
+    for s, c in enumerate(n):
+        for j in range(31, c, 32):
+            pool.v[int(pool.table[s, j // 16]), j % 16, :, j // 32 % dim] = float("nan")
+            want[starts(n)[s] + j:starts(n)[s + 1], j // 32 % dim] = True
+    o = voxq.paged_attention(q, pool.k, pool.v, *args)
+    assert int(voxq.lib().voxq_device_error(1)) == 0
+    assert torch.equal(torch.isnan(o).cpu(), want[:, None].expand(-1, 16, -1))
+    # p rounded or not, the output rounded: 2^-8 of the value and 2^-8 of what the weights' errors move
+    off = (o.float() - clean.float()).abs().cpu()[~torch.isnan(o).cpu()]
+    size = clean.float().abs().cpu()[~torch.isnan(o).cpu()]
+    assert (off <= 2.0 ** -7 * (size + 1.0)).all()

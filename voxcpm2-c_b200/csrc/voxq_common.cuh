@@ -199,9 +199,9 @@ __device__ __forceinline__ bool mbar_try_wait_suspend(uint64_t* bar, uint32_t pa
     return ok != 0;
 }
 
-// Waits for a barrier phase for at most `limit` suspended polls of up to
-// 1 ms each (about a second); returns false and records `site` when the phase
-// never completes.  A waiting warp is parked by the hardware, so waiting costs
+// Waits for a barrier phase for at most `limit` suspended polls, which may
+// last 1 ms each and were measured at 4 us (so 4 ms by default); returns false
+// and records `site` when the phase never completes.  A waiting warp is parked by the hardware, so waiting costs
 // no issue slots of the warps doing the work.
 __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, int site, int* err,
                                                   uint32_t limit = 1000u) {

@@ -22,7 +22,6 @@ constexpr int kTcHalf = kTcTile * 128;       // bytes of 128 rows x 64 dims, 128
 constexpr int kTcTails = 3;
 constexpr int kTcItems = 4;                  // units in flight between the warps of a block
 constexpr int kTcSeqs = 4;                   // of 32 sequences: up to how many the units are taken in order of their keys
-constexpr uint32_t kTcLong = 20000;           // limit (ms) of the waits that span a whole unit of work
 constexpr float kTcSlack = 8.0f;             // how far a row's maximum may grow (log2) before its sums are rescaled
 template <int HD>
 constexpr int kTcTileBytes = kTcHalf * (HD / 64);
@@ -137,6 +136,21 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
         const __half2 v = __floats2half2_rn(x, y);
         return *reinterpret_cast<const uint32_t*>(&v);
     }
+}
+
+// The waits that span a whole unit of work, which lasts as long as its keys are many: bounded by the clock, 20 seconds.  (A poll
+// of mbar_wait_bounded takes some 4 us: 20 000 of them end after 80 ms, the time of some 4 million keys.)
+__device__ __forceinline__ bool wait_unit(uint64_t* bar, uint32_t parity, int site, int* err) {
+    uint64_t from = 0, now;
+#pragma unroll 1
+    while (!mbar_try_wait_suspend(bar, parity, 1000000u)) {
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+        if (from == 0) from = now;
+        const bool late = now - from > 20000000000ull;
+        if (late) atomicCAS(err, 0, site);
+        if (late || *reinterpret_cast<volatile int*>(err) != 0) return false;  // this wait or another gave up
+    }
+    return true;
 }
 
 // A bounded wait whose answer is the same for the whole warp.
@@ -258,7 +272,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
 
     // The k-th unit; rows 0: no more.  done(k) frees its slot.
     auto unit_ready = [&](int k) {
-        return __all_sync(0xffffffffu, mbar_wait_bounded(item_full + k % kTcItems, (k / kTcItems) & 1, VOXQ_DEVERR_WAIT_FULL, p.err, kTcLong));
+        return __all_sync(0xffffffffu, wait_unit(item_full + k % kTcItems, (k / kTcItems) & 1, VOXQ_DEVERR_WAIT_FULL, p.err));
     };
     auto done = [&](int k) {
         __syncwarp();
@@ -581,7 +595,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
                     for (int t = 0; t < TW; t++) {
                         if (t && !two) break;
-                        ok = ok && mbar_wait_bounded(q_full + t, units[t]++ & 1, VOXQ_DEVERR_WAIT_FULL, p.err, kTcLong);
+                        ok = ok && wait_unit(q_full + t, units[t]++ & 1, VOXQ_DEVERR_WAIT_FULL, p.err);
                         tc_after();
                         if (ok) scores(t, sk);
                     }
@@ -641,7 +655,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             int x = blockIdx.x, y, z = blockIdx.z, k = 0;
             bool ok = true;
             auto put = [&](const TcItem& it) {
-                if (k >= kTcItems) ok = __all_sync(0xffffffffu, mbar_wait_bounded(item_empty + k % kTcItems, (k / kTcItems - 1) & 1, VOXQ_DEVERR_WAIT_EMPTY, p.err, kTcLong));
+                if (k >= kTcItems) ok = __all_sync(0xffffffffu, wait_unit(item_empty + k % kTcItems, (k / kTcItems - 1) & 1, VOXQ_DEVERR_WAIT_EMPTY, p.err));
                 if (lane == 0 && ok) {
                     items[k % kTcItems] = it;
                     mbar_arrive(item_full + k % kTcItems);
@@ -732,7 +746,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                         put(it);
                         // No unit is taken before the loader has come to this one: a block that reserved more would sit on
                         // them while others run out of work.
-                        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(begun, (k - 1) & 1, VOXQ_DEVERR_WAIT_EMPTY, p.err, kTcLong));
+                        ok = ok && __all_sync(0xffffffffu, wait_unit(begun, (k - 1) & 1, VOXQ_DEVERR_WAIT_EMPTY, p.err));
                         if (!ok) break;
                     }
                 }
@@ -752,7 +766,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             // (the kernel's last code: between the others' it took 10 us more from cold caches)
             for (int k = 0; unit_ready(k) && items[k % kTcItems].rows > 0; k++) {
                 const TcItem& it = items[k % kTcItems];
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(written + k % kTcItems, (k / kTcItems) & 1, VOXQ_DEVERR_WAIT_FULL, p.err, kTcLong))) break;
+                if (!__all_sync(0xffffffffu, wait_unit(written + k % kTcItems, (k / kTcItems) & 1, VOXQ_DEVERR_WAIT_FULL, p.err))) break;
                 RowsAgain<T> found(it.k_beg);
                 for (int w = 0; w < 8; w++)
                     for (uint32_t rows = again[k % kTcItems][w]; rows; rows &= rows - 1) {

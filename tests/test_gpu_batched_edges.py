@@ -8,7 +8,7 @@ import pytest
 torch = pytest.importorskip("torch")
 import batched_ref as R  # noqa: E402
 import voxq  # noqa: E402
-from test_gpu_batched import BF16, F16, F32, Pool, ids, ints, starts  # noqa: E402
+from test_gpu_batched import BF16, F16, F32, LORA_TYPES, Pool, ids, ints, lora_inputs, starts  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -190,3 +190,21 @@ def test_units_of_work_that_last_long():
     off = (o.float() - clean.float()).abs().cpu()[~torch.isnan(o).cpu()]
     size = clean.float().abs().cpu()[~torch.isnan(o).cpu()]
     assert (off <= 2.0 ** -7 * (size + 1.0)).all()
+
+
+@pytest.mark.parametrize("dt,wt", LORA_TYPES, ids=ids)
+@pytest.mark.parametrize("rows", [[5, 1], [9000, 3]], ids=["few", "many"])
+def test_lora_keeps_a_nan_in_its_weights(rows, dt, wt):
+    """One in A reaches every column of its request, one in B its own column; whatever its bits."""
+    x, a, b, cu, _, scale, base = lora_inputs(rows, 2, 264, 520, 40, dt, wt, seed=6)
+    clean = voxq.lora(x, a, b, cu, ints([0, 1]), scale, base=base)
+    b[0, 300, 2] = float("nan")
+    b[1].view(torch.int32 if wt is F32 else torch.int16)[7, 0] = 0x7fffffff if wt is F32 else 0x7fff
+    y = voxq.lora(x, a, b, cu, ints([0, 1]), scale, base=base)
+    want = torch.zeros_like(y, dtype=torch.bool)
+    want[:rows[0], 300], want[rows[0]:, 7] = True, True
+    assert torch.equal(torch.isnan(y), want) and torch.equal(y[~want], clean[~want])
+    a[0].view(torch.int32 if wt is F32 else torch.int16)[39, 263] = 0x7fffffff if wt is F32 else 0x7fff
+    y = voxq.lora(x, a, b, cu, ints([0, 1]), scale, base=base)
+    want[:rows[0]] = True
+    assert torch.equal(torch.isnan(y), want)

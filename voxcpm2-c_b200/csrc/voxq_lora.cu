@@ -77,8 +77,13 @@ __device__ __forceinline__ void mul_16(float (*d)[4], const T* as, const T* as_l
                 if (i >= blocks) break;
                 const W* br = bs + (i * 8 + g) * bp + k + t;
                 uint32_t bh[2], bl[2];
-                split_tf32(to_f(br[0]), bh[0], bl[0]);
-                split_tf32(to_f(br[4]), bh[1], bl[1]);
+                if constexpr (is_f32<W>) {
+                    split_tf32(br[0], bh[0], bl[0]);
+                    split_tf32(br[4], bh[1], bl[1]);
+                } else {  // as it is: rounding would carry a NaN of nothing but ones over into a zero
+                    bh[0] = __float_as_uint(to_f(br[0]));
+                    bh[1] = __float_as_uint(to_f(br[4]));
+                }
                 mma8(d[i], al, bh[0], bh[1]);
                 if (is_f32<W>) mma8(d[i], ah, bl[0], bl[1]);
                 mma8(d[i], ah, bh[0], bh[1]);

@@ -607,7 +607,9 @@ VOXQ_API VoxCPMError voxq_paged_attention(const voxq_paged_attn* d, void* stream
  * base NULL counts as zeros; out may be base.  x, base and out are one type;
  * A and B are that type, or any of the three for fp32 x.  16-byte rows; K, N
  * and rank multiples of 8, rank <= 128.  cu[batch] is rows: a row that no request owns is not
- * written.  In fp16, scale (x A^T) must lie in fp16's range. */
+ * written.  In fp16, scale (x A^T) must lie in fp16's range.  Infinities and NaN
+ * count as in the formula, but that an infinity in B (in fp32 any value from
+ * 3.402e38 on) may come out as a NaN. */
 typedef struct {
     const void* x;
     int64_t ldx;

@@ -208,3 +208,37 @@ def test_lora_keeps_a_nan_in_its_weights(rows, dt, wt):
     y = voxq.lora(x, a, b, cu, ints([0, 1]), scale, base=base)
     want[:rows[0]] = True
     assert torch.equal(torch.isnan(y), want)
+
+
+@pytest.mark.parametrize("dt,wt", LORA_TYPES, ids=ids)
+@pytest.mark.parametrize("rank", [8, 24, 40, 72])
+@pytest.mark.parametrize("rows", [[5, 3, 1, 4], [4000, 900, 3, 700]], ids=["few", "many"])
+def test_lora_that_meets_infinities_and_nan(rows, rank, dt, wt):
+    """Infinite and NaN inputs, weights and hidden values give what the formula gives, and harm no other row or column."""
+    K, N = 264, 520
+    x, a, b, cu, _, scale, base = lora_inputs(rows, 4, K, N, rank, dt, wt, seed=9)
+    who, ranks = ints([0, 1, 2, 3]), ints([rank, rank - 3, rank, rank])
+    inf, nan = float("inf"), float("nan")
+    top = torch.finfo(dt).max
+    a[0, :, 5], b[0, :40] = a[0, :, 5].abs() + 0.01, b[0, :40].abs() + 0.01
+    a[0, :, 11] = 2e-38 if wt is F32 else 0       # beside a value next to the type's end: a small product, or nothing
+    x[0, 11], x[1, 5], x[2, 5], x[3, 7], x[4, 100] = top, inf, -inf, nan, inf
+    b[1, 9, 1], b[1, 10, 0], b[1, 300, 2] = inf, -inf, nan
+    a[1, rank - 3:], b[1, :, rank - 3:] = nan, inf   # past the adapter's own rank
+    a[2, 3, 9] = inf
+    base[rows[0], 17] = inf
+    bound_of = [torch.nan_to_num(t, 0, 0, 0) for t in (x, a, b, base)]
+    _, bound = R.adapters(bound_of[0], bound_of[1], bound_of[2], cu, who, scale, bound_of[3], ranks)
+    y = R.f8(voxq.lora(x, a, b, cu, who, scale, base=base, ranks=ranks))
+    ref = R.f8(base).clone()
+    for s, r in enumerate(ranks.tolist()):
+        at = slice(int(cu[s]), int(cu[s + 1]))
+        ref[at] += float(scale[s]) * (R.f8(x[at]) @ R.f8(a[s, :r]).T @ R.f8(b[s, :, :r]).T)
+    at = torch.zeros_like(ref, dtype=torch.bool)  # an infinity in B may come out as a NaN
+    at[rows[0]:rows[0] + rows[1], 9:11] = True
+    assert not torch.isfinite(ref[at]).any()
+    ref[at & torch.isnan(y)] = nan
+    assert torch.equal(torch.isnan(y), torch.isnan(ref)), "NaN in other places than the formula's"
+    fine = torch.isfinite(ref)
+    assert torch.equal(y[~fine & ~torch.isnan(ref)], ref[~fine & ~torch.isnan(ref)]), "infinities in other places than the formula's"
+    R.assert_within(torch.where(fine, y, 0.0), torch.where(fine, ref, 0.0), bound)

@@ -56,6 +56,21 @@ inline cudaError_t launch_pdl(void (*kern)(P...), dim3 grid, dim3 block, size_t 
 template <typename T>
 constexpr bool is_f32 = std::is_same<T, float>::value;
 
+// Four elements of a 16-byte row as fp32.
+template <typename T>
+__device__ __forceinline__ void load4(float (&x)[4], const T* p) {
+    T e[4];
+    if constexpr (is_f32<T>) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        memcpy(e, &v, 16);
+    } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        memcpy(e, &v, 8);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = to_f(e[i]);
+}
+
 // 16 bytes to shared memory, zeros when !ok (the source is then not read).
 __device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool ok) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0) : "memory");

@@ -121,6 +121,25 @@ __device__ __forceinline__ void load_b(W* dst, int bp, const W* b, int n0, int N
     }
 }
 
+// A sum that products in two TF32 parts did not leave finite, once more in plain fp32: the parts of an infinity, or of an fp32
+// value that rounds to one, make a NaN (inf - inf, 0 * inf).  What is not finite here is so by the formula.  x and a are rows of
+// whole fours, a's past K whatever they may be.  (An infinity in B meets h's parts in every column step; looking for it there
+// took the prompts 13 % more time in bf16 and 7 % in fp32.)
+template <typename W>
+__device__ __forceinline__ float plain_sum(const float* x, const W* a, int K) {
+    float v = 0.0f;
+#pragma unroll 1
+    for (int k = 0; k < K && v == v; k += 4) {
+        float p[4], w[4];
+        load4(p, x + k);
+        load4(w, a + k);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (k + e < K) v = fmaf(p[e], w[e], v);
+    }
+    return v;
+}
+
 // One cluster per tile of up to TM rows of one request, both products in one
 // launch.  The CTAs of the cluster split K for h = x A^T (chunks of KB, two
 // cp.async stages), add their partial sums of h through each other's shared
@@ -167,6 +186,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
     W* bs0 = reinterpret_cast<W*>(lora_sh + z.o_b0);
     T* hs = reinterpret_cast<T*>(lora_sh + z.o_hs);  // h as two 16-bit parts, or fp32
     T* hs_lo = hs + (is_f32<T> ? 0 : TM * z.hp);
+    bool plain = false;  // h is not finite somewhere, which two parts of it would not survive
     if (r > 0) {
         load_b<W, NB, NW>(bs0, z.bp, wb, crank * NB, d.N, d.rank, r, per, inv);
         cp_async_commit();
@@ -250,7 +270,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
         for (int i = threadIdx.x; i < TM * (z.Rp / 4); i += kLoraThreads) {
             const int row = i / (z.Rp / 4), col = i % (z.Rp / 4) * 4;
             float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (row < rows && col < r)
+            if (row < rows && col < r) {
                 for (uint32_t c = 0; c < csize; c++) {
                     uint32_t addr;
                     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(local + (row * z.hp + col) * 4), "r"(c));
@@ -260,15 +280,27 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
 #pragma unroll
                     for (int j = 0; j < 4; j++) v[j] += p[j];
                 }
+                if constexpr (is_f32<T>) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (v[j] - v[j] != 0.0f && col + j < r)
+                            v[j] = plain_sum((const T*)d.x + (m0 + row) * d.ldx, wa + (int64_t)(col + j) * d.K, d.K);
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const float h = col + j < r ? v[j] * scale : 0.0f;
                 hs[row * z.hp + col + j] = from_f<T>(h);
-                if constexpr (!is_f32<T>) hs_lo[row * z.hp + col + j] = from_f<T>(h - to_f(from_f<T>(h)));
+                if (is_f32<T>) plain = plain || !(fabsf(h) < 3.4e38f);
+                if constexpr (!is_f32<T>) {
+                    const float hi = to_f(from_f<T>(h));
+                    hs_lo[row * z.hp + col + j] = from_f<T>(hi - hi == 0.0f ? h - hi : 0.0f);  // (an infinity has no rest)
+                }
             }
         }
         // peers may still read this CTA's part: no CTA leaves before all have arrived here
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        if constexpr (is_f32<T>) plain = __syncthreads_or(plain);
     }
 
     // Columns n0 .. n0 + NB - 1 at a time; a warp owns 16 rows x NW columns of them, a thread CW neighbours of rows g and
@@ -291,7 +323,7 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
     uint4 old[2][VC], next[2][VC];
     fetch_base(crank * NB, old);
     int it = 0;
-    for (int n0 = crank * NB; n0 < d.N; n0 += step, it++) {
+    for (int n0 = crank * NB; n0 < d.N && !plain; n0 += step, it++) {
         fetch_base(n0 + step, next);
         float o[NW / 8][4];
 #pragma unroll
@@ -325,6 +357,15 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
 #pragma unroll
             for (int j = 0; j < VC; j++) old[e][j] = next[e][j];
     }
+    if constexpr (is_f32<T>)
+        if (plain)
+            for (int n0 = crank * NB; n0 < d.N; n0 += step)
+                for (int i = threadIdx.x; i < rows * NB; i += kLoraThreads) {
+                    const int row = i / NB, n = n0 + i % NB;
+                    if (n >= d.N) continue;
+                    const float base = d.base ? ((const float*)d.base)[(m0 + row) * d.ldb + n] : 0.0f;
+                    ((float*)d.out)[(m0 + row) * d.ldo + n] = base + plain_sum((const T*)hs + row * z.hp, wb + (int64_t)n * d.rank, r);
+                }
     cp_async_wait<0>();
     if (r > 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

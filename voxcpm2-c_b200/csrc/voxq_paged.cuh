@@ -235,21 +235,6 @@ __device__ __forceinline__ void attend_keys(const PagedArgs& p, const T* qs, con
     }
 }
 
-// Four elements of a 16-byte row as fp32.
-template <typename T>
-__device__ __forceinline__ void load4(float (&x)[4], const T* p) {
-    T e[4];
-    if constexpr (is_f32<T>) {
-        const float4 v = *reinterpret_cast<const float4*>(p);
-        memcpy(e, &v, 16);
-    } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        memcpy(e, &v, 8);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = to_f(e[i]);
-}
-
 // What the matrix instructions get wrong where something is not finite, put right by a warp.  Operands and weights in two
 // parts turn an infinity (and an fp32 value that rounds to one) into a NaN, inf - inf or 0 * inf, and a key that only some of
 // a tile's rows see has the weight 0 in the others, where 0 * NaN and 0 * inf are NaN.  So the rows whose sums came out that

@@ -405,8 +405,10 @@ static VoxCPMError lora_launch(const voxq_lora& d, cudaStream_t st) {
 // their operands for every MMA and want the more warps a row unless the rank is high.  us, 64 against 16 rows, bf16, rank 32,
 // K 1024, N 4096: 40 requests of 64 rows 35 : 31, of 128 49 : 51, of 300 80 : 104; 2 of 4096 47 : 55; rank 64, N 1024: 9 of
 // 1000 37 : 53.  fp32, rank 16, K = N = 2048: 9 of 1000 84 : 68, 2 of 4096 92 : 68; rank 64, K 1024, N 2048: 9 of 1000 123 : 150,
-// 40 of 300 227 : 219; bf16, rank 64, K 2960, N 1032: 30 of 96 37 : 51, 40 of 64 37 : 33, 4 of 40 22 : 16.  Steps of 256 columns where they keep the eight CTAs of a cluster busy, of 128 else: 40 single rows,
-// N 2048, 8.3 : 9.8; N 1024, 18 : 16.
+// 40 of 300 227 : 219; bf16, rank 64, K 2960, N 1032: 30 of 96 37 : 51, 40 of 64 37 : 33, 4 of 40 22 : 16.
+// Steps of 256 columns for 16-row tiles so few that eight CTAs share each, of whom every one still gets a step: they pay each step's
+// wait less often.  Of 128 else, where the fewer registers count.  us, 256 : 128, K 2048, rank 16, fp32 x with bf16 weights: 40 single
+// rows, N 1024 8.0 : 8.0, N 2048 8.2 : 9.5, N 4096 9.6 : 12.4; 9 of 1000 rows, N 1024 63 : 48, N 2048 90 : 69, N 4096 141 : 112.
 template <typename T, typename W>
 static VoxCPMError lora_dispatch(const voxq_lora& d, cudaStream_t st) {
     const bool tall = d.rows >= 24 * (int64_t)d.batch && d.rows >= (d.rank > 32 && !is_f32<T> ? 16 : 32) * device_sm_count();
@@ -414,7 +416,8 @@ static VoxCPMError lora_dispatch(const voxq_lora& d, cudaStream_t st) {
     if (d.rank > 32) return tall ? lora_launch<T, W, 64, 8, 64>(d, st) : lora_launch<T, W, 16, 8, 128>(d, st);
     if constexpr (!is_f32<T>)
         if (tall) return lora_launch<T, W, 64, 4, 64>(d, st);
-    return d.N >= 2048 ? lora_launch<T, W, 16, 4, 256>(d, st) : lora_launch<T, W, 16, 4, 128>(d, st);
+    const bool eight = d.rows / 16 + d.batch <= 4 * device_sm_count() / 8;
+    return eight && d.N >= 8 * 256 ? lora_launch<T, W, 16, 4, 256>(d, st) : lora_launch<T, W, 16, 4, 128>(d, st);
 }
 
 }  // namespace voxq

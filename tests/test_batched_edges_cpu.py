@@ -123,3 +123,9 @@ def test_the_binding_is_rebuilt_for_another_torch(tmp_path, monkeypatch):
     assert m.build_binding() and len(ran) == 1
     monkeypatch.setattr(torch, "__version__", "0.0.another")
     assert m.build_binding() and len(ran) == 2
+
+
+def test_an_output_of_another_type_than_asked_for_is_refused():
+    z = torch.zeros
+    with pytest.raises(ValueError, match="differ"):
+        voxq.paged_attention(z(1, 4, 64), z(2, 16, 2, 64), z(2, 16, 2, 64), None, None, None, 1, 16, out=z(1, 4, 64), out_dtype=torch.float16)

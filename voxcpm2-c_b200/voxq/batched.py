@@ -88,6 +88,7 @@ def paged_attention(q, cache_k, cache_v, block_table, cu_q, kv_len, max_q: int, 
     if stream is not None:
         with _on(stream, _device(q)):
             return paged_attention(q, cache_k, cache_v, block_table, cu_q, kv_len, max_q, max_kv, causal, scale, out, out_dtype)
+    _need(out is None or out_dtype is None or out.dtype == out_dtype, "out and out_dtype differ")
     if out is None and out_dtype is not None:
         out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
     return _torch.paged_attention(q, cache_k, cache_v, block_table, cu_q, kv_len, max_q, max_kv, causal, scale, out)

@@ -99,6 +99,14 @@ int i32(int64_t v) {
 }
 void* stream_of(const at::Tensor& like) { return (void*)c10::cuda::getCurrentCUDAStream(like.get_device()).stream(); }
 
+// Makes a tensor's GPU the current one.  (It mostly is, and a guard asks three times.)
+struct Here {
+    c10::cuda::OptionalCUDAGuard guard;
+    explicit Here(const at::Tensor& like) {
+        if (like.get_device() != c10::cuda::current_device()) guard.set_device(like.device());
+    }
+};
+
 // Memory of the current stream, contiguous, without the dispatcher's half microsecond a tensor.
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
     return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
@@ -139,7 +147,7 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
              "q [T, heads, D] and k, v [T, kv_heads, D] of one type are needed");
         caches(ck, cv, D);
         need(ck.size(2) == KVH, "the caches' kv_heads differ from k's");
-        const c10::cuda::CUDAGuard here(q.device());
+        const Here here(q);
         at::Tensor out = given ? *given : fresh(q.sizes(), ck.scalar_type(), q);
         need(rows_ok(out, 3) && out.sizes() == q.sizes() && out.scalar_type() == ck.scalar_type(), "q_out: q's shape and the caches' type, on the GPU");
         voxq_rope d{};
@@ -198,7 +206,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         d.max_q = as_i32(a[6], "max_q is past 2^31");
         d.max_kv = as_i32(a[7], "max_kv is past 2^31");
         need(d.max_kv <= bt.size(1) * ck.size(1), "max_kv is more than the block table's pages hold");
-        const c10::cuda::CUDAGuard here(q.device());
+        const Here here(q);
         at::Tensor out = given ? *given : fresh(q.sizes(), q.scalar_type(), q);
         need(rows_ok(out, 3) && out.sizes() == q.sizes(), "out: q's shape, contiguous along head_dim, on the GPU");
         d.q = q.const_data_ptr();
@@ -253,7 +261,7 @@ PyObject* lora(PyObject*, PyObject* const* o, Py_ssize_t n) {
         const int64_t M = x.size(0), N = b.size(1), B = who.numel(), nA = a.size(0);
         auto fits = [&](const at::Tensor& t) { return rows_ok(t, 2) && t.size(0) == M && t.size(1) == N && t.scalar_type() == x.scalar_type(); };
         need(!base || fits(*base), "base: [rows, N] of x's type, contiguous along N, on the GPU");
-        const c10::cuda::CUDAGuard here(x.device());
+        const Here here(x);
         at::Tensor out = given ? *given : fresh({M, N}, x.scalar_type(), x);
         need(fits(out), "out: [rows, N] of x's type, contiguous along N, on the GPU");
         voxq_lora d{};
@@ -297,7 +305,7 @@ PyObject* norm_residual(PyObject*, PyObject* const* a, Py_ssize_t n) {
         need(fits(x), "y and x: [rows, D] of one type, contiguous along D, on the GPU");
         need(w_pre || !n_given, "n_out needs w_pre");
         const int64_t M = y.size(0), D = y.size(1);
-        const c10::cuda::CUDAGuard here(y.device());
+        const Here here(y);
         voxq_norm d{};
         if (gate) {
             need(rows_ok(*gate, 2) && gate->size(1) == D && gate->scalar_type() == y.scalar_type(),

@@ -402,10 +402,11 @@ static VoxCPMError lora_launch(const voxq_lora& d, cudaStream_t st) {
 }
 
 // Tiles of 64 rows read the weights less often and pay where there are enough of them and few are part empty; fp32 rows split
-// their operands for every MMA and want the more warps a row unless the rank is high.  us, 64 against 16 rows, bf16, rank 32,
-// K 1024, N 4096: 40 requests of 64 rows 35 : 31, of 128 49 : 51, of 300 80 : 104; 2 of 4096 47 : 55; rank 64, N 1024: 9 of
-// 1000 37 : 53.  fp32, rank 16, K = N = 2048: 9 of 1000 84 : 68, 2 of 4096 92 : 68; rank 64, K 1024, N 2048: 9 of 1000 123 : 150,
-// 40 of 300 227 : 219; bf16, rank 64, K 2960, N 1032: 30 of 96 37 : 51, 40 of 64 37 : 33, 4 of 40 22 : 16.
+// their operands for every MMA and want the more warps a row unless the rank is high.  us, 64 against 16 rows.  bf16, rank 32,
+// K 1024, N 4096: 40 requests of 64 rows 31 : 29, of 128 43 : 53, of 300 81 : 91, 2 of 4096 50 : 58; rank 64, K 2960, N 1032: 30 of
+// 96 32 : 45, 40 of 64 32 : 44, 4 of 40 17 : 13; rank 128, K 1024, N 2048: 9 of 1000 115 : 196.  fp32 x, K 1024, N 2048, bf16 weights, rank
+// 64: 9 of 1000 91 : 109, 40 of 300 169 : 160, of 128 85 : 106; rank 128: 9 of 1000 237 : 326.  fp32 weights: rank 48 106 : 127, rank 64
+// 182 : 155 (the one class whose tall tiles lose), rank 128 302 : 445.
 // Steps of 256 columns for 16-row tiles so few that eight CTAs share each, of whom every one still gets a step: they pay each step's
 // wait less often.  Of 128 else, where the fewer registers count.  us, 256 : 128, K 2048, rank 16, fp32 x with bf16 weights: 40 single
 // rows, N 1024 8.0 : 8.0, N 2048 8.2 : 9.5, N 4096 9.6 : 12.4; 9 of 1000 rows, N 1024 63 : 48, N 2048 90 : 69, N 4096 141 : 112.

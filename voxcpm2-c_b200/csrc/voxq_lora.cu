@@ -370,6 +370,19 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const __grid_constan
     if (r > 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// As many tiles as the requests can need.
+static int lora_tiles(const voxq_lora& d, int rows) { return d.rows / rows + d.batch; }
+
+// As many CTAs to a tile as keep the grid within 4 an SM, up to 8.  Where 4 fit an SM any number, else a power of two, which
+// leaves no holes in a second round.  bf16 prompts (8000 rows, K 1024, N 4096, rank 32): 42 us, 47 with powers of two, 71
+// with a bound of 2 an SM and 50 with 8; 9 of 1000 rows, rank 64, K 2960, N 1032: 59 us, 78 with any number.
+static int lora_cluster(int tiles, int bytes) {
+    int cl = std::min(8, std::max(1, 4 * device_sm_count() / tiles));
+    if (bytes + 1024 > 227 * 1024 / 4)
+        while (cl & (cl - 1)) cl--;
+    return cl;
+}
+
 template <typename T, typename W, int TM, int RB, int COLS>
 static VoxCPMError lora_launch(const voxq_lora& d, cudaStream_t st) {
     using S = LoraShape<T, W, TM, COLS>;
@@ -377,13 +390,7 @@ static VoxCPMError lora_launch(const voxq_lora& d, cudaStream_t st) {
     auto kern = lora_kernel<T, W, TM, RB, COLS>;
     static std::atomic<uint64_t> asked{0};
     VOXQ_CUDA_TRY(allow_shared((const void*)kern, S(RB * 8).bytes, asked));
-    // As many CTAs to a tile as keep the grid within 4 an SM, up to 8.  Where 4 fit an SM any number, else a power of two, which
-    // leaves no holes in a second round.  bf16 prompts (8000 rows, K 1024, N 4096, rank 32): 42 us, 47 with powers of two, 71
-    // with a bound of 2 an SM and 50 with 8; 9 of 1000 rows, rank 64, K 2960, N 1032: 59 us, 78 with any number.
-    const int tiles = d.rows / TM + d.batch;
-    int cl = std::min(8, std::max(1, 4 * device_sm_count() / tiles));
-    if (z.bytes + 1024 > 227 * 1024 / 4)
-        while (cl & (cl - 1)) cl--;
+    const int tiles = lora_tiles(d, TM), cl = lora_cluster(tiles, z.bytes);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles * cl);
     cfg.blockDim = dim3(kLoraThreads);
@@ -407,9 +414,11 @@ static VoxCPMError lora_launch(const voxq_lora& d, cudaStream_t st) {
 // 96 32 : 45, 40 of 64 32 : 44, 4 of 40 17 : 13; rank 128, K 1024, N 2048: 9 of 1000 115 : 196.  fp32 x, K 1024, N 2048, bf16 weights, rank
 // 64: 9 of 1000 91 : 109, 40 of 300 169 : 160, of 128 85 : 106; rank 128: 9 of 1000 237 : 326.  fp32 weights: rank 48 106 : 127, rank 64
 // 182 : 155 (the one class whose tall tiles lose), rank 128 302 : 445.
-// Steps of 256 columns for 16-row tiles so few that eight CTAs share each, of whom every one still gets a step: they pay each step's
-// wait less often.  Of 128 else, where the fewer registers count.  us, 256 : 128, K 2048, rank 16, fp32 x with bf16 weights: 40 single
-// rows, N 1024 8.0 : 8.0, N 2048 8.2 : 9.5, N 4096 9.6 : 12.4; 9 of 1000 rows, N 1024 63 : 48, N 2048 90 : 69, N 4096 141 : 112.
+// Steps of 256 columns pay each step's wait less often, but their registers leave an SM three blocks: taken where all blocks then
+// run at once (a request that is shorter than a tile has one tile all the same) and have a step each.  us, 256 against 128 columns, fp32 x, bf16 weights, rank 16, K 2048, N 2048: 40 single rows 8.2 : 9.5, 40
+// requests of 8 9.7 : 11.1, of 64 26 : 30; not all at once: 100 single rows 18.8 : 15.2, 3 of 300 19 : 14, 9 of 1000 90 : 69.  Rank
+// 32, where clusters are powers of two: 100 single rows 15.3 : 18.5.  bf16 x: 40 of 8 7.7 : 8.6, 3 of 300 13.8 : 9.6.  N 1024: 20 single rows,
+// rank 32, 8.5 : 7.3.
 template <typename T, typename W>
 static VoxCPMError lora_dispatch(const voxq_lora& d, cudaStream_t st) {
     const bool tall = d.rows >= 24 * (int64_t)d.batch && d.rows >= (d.rank > 32 && !is_f32<T> ? 16 : 32) * device_sm_count();
@@ -417,8 +426,8 @@ static VoxCPMError lora_dispatch(const voxq_lora& d, cudaStream_t st) {
     if (d.rank > 32) return tall ? lora_launch<T, W, 64, 8, 64>(d, st) : lora_launch<T, W, 16, 8, 128>(d, st);
     if constexpr (!is_f32<T>)
         if (tall) return lora_launch<T, W, 64, 4, 64>(d, st);
-    const bool eight = d.rows / 16 + d.batch <= 4 * device_sm_count() / 8;
-    return eight && d.N >= 8 * 256 ? lora_launch<T, W, 16, 4, 256>(d, st) : lora_launch<T, W, 16, 4, 128>(d, st);
+    const int64_t blocks = (int64_t)std::max(d.batch, d.rows / 16) * lora_cluster(lora_tiles(d, 16), LoraShape<T, W, 16, 256>(d.rank).bytes);
+    return d.N >= 8 * 256 && blocks <= 3 * device_sm_count() ? lora_launch<T, W, 16, 4, 256>(d, st) : lora_launch<T, W, 16, 4, 128>(d, st);
 }
 
 }  // namespace voxq

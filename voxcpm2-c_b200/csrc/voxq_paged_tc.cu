@@ -214,12 +214,12 @@ __device__ __forceinline__ bool next_block(const uint4* answer, int& x, int& y, 
 // A block stays for many units (the grid is one block per unit; the running ones take over the rest): the loader and
 // the first scores of a unit run ahead of the previous one's output, and tensor memory, barriers and shared memory are
 // set up once.  Every wait is bounded and records the device error word.
-// 6 causal prompts of 1500..4096 tokens, 16 query heads over 2 kv heads x 128, bf16 (279 GFLOP): 285 us in a short burst,
-// 0.98 PFLOP/s; 315 us over and over, when the power limit lowers the clocks.  (One block a unit, in the order of the batch,
+// 6 causal prompts of 1500..4096 tokens, 16 query heads over 2 kv heads x 128, bf16 (279 GFLOP): 322 us over and over, 0.87
+// PFLOP/s, when the power limit lowers the clocks; 289 us where a few calls follow one another.  (One block a unit, in the order of the batch,
 // with a maximum before the weights: 380 us.)  Bound by the chain of a key tile: the softmax warps wait 1300 clocks for the
 // scores, read them in 70, take 1450 for maximum, exponentials (at 16 a clock an SM alone 1024 for both tiles) and
 // rounding, 220 to write the weights; a unit's output and next queries add 8500.  One or two tiles that fill the machine
-// once (3 sequences of 40..64 tokens on 12 000 keys: 37 us) pay that start and end and the join for one short run.
+// once (3 sequences of 40..64 tokens on 12 000 keys: 38 us) pay that start and end and the join for one short run.
 template <typename T, int HD, bool LOW>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ PagedArgs p, const __grid_constant__ PagedMaps maps) {
     constexpr int TILE = kTcTileBytes<HD>, ST = kTcStages<HD>, TW = kTcTiles<HD>, ROWS = TW * kTcTile;

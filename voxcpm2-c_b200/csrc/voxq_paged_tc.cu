@@ -148,7 +148,8 @@ __device__ __forceinline__ bool wait_unit(uint64_t* bar, uint32_t parity, int si
         if (from == 0) from = now;
         const bool late = now - from > 20000000000ull;
         if (late) atomicCAS(err, 0, site);
-        if (late || *reinterpret_cast<volatile int*>(err) != 0) return false;  // this wait or another gave up
+        // this wait or another gave up (an error of an earlier call stops no wait that goes on as it should)
+        if (late || (now - from > 20000 && *reinterpret_cast<volatile int*>(err) != 0)) return false;
     }
     return true;
 }

@@ -117,13 +117,18 @@ __device__ __forceinline__ uint32_t pack2v(float x, float y) {  // x in the low 
     return r;
 }
 
-// What pack2v's r leaves of x and y, in the same type.
+// pack2v's r as fp32 again, and what it leaves of x and y, in the same type.
 template <typename T>
-__device__ __forceinline__ uint32_t rest2v(uint32_t r, float x, float y) {
+__device__ __forceinline__ uint64_t both_f(uint32_t r) {
+    if constexpr (std::is_same<T, bf16>::value) return pk(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
     T e[2];
     memcpy(e, &r, 4);
+    return pk(to_f(e[0]), to_f(e[1]));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t rest2v(uint32_t r, float x, float y) {
     float a, b;
-    upk(fma2v(pk(to_f(e[0]), to_f(e[1])), pk(-1.0f, -1.0f), pk(x, y)), a, b);
+    upk(fma2v(both_f<T>(r), pk(-1.0f, -1.0f), pk(x, y)), a, b);
     return pack2v<T>(a, b);
 }
 
@@ -208,7 +213,7 @@ __device__ __forceinline__ bool next_block(const uint4* answer, int& x, int& y, 
 // p.  For a 16-bit output p is rounded once to the operand type: that moves the output by 0.0006 of its norm in bf16, where its
 // own rounding moves it by 0.0017, and a second part takes a quarter more time (the prompts below 356 us for 285).  An fp32
 // output has no rounding to hide behind: there p enters the second product as two 16-bit parts (LOW; 305 us with one part and
-// an error of 2^-9.6 of the norm, 372 with two and under 2^-13).
+// an error of 2^-9.6 of the norm, 356 with two and under 2^-13).
 // Head dims below HD are zeros in shared memory: the tensor maps end there, and the queries are written so.  HD 256: one
 // query tile a unit and a ring of two, so that a tile's softmax waits for its products and they for it; 4 prompts of 300
 // tokens on 1000 keys 111 us, 0.2 PFLOP/s, where the MMA kernel takes 252.
@@ -388,9 +393,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                         }
                         if (c >= BEHIND) {
                             const int o = c - BEHIND;
-                            sum[o & 1] = add2v(sum[o & 1], pk(y[2 * o], y[2 * o + 1]));
+                            if (!LOW) sum[o & 1] = add2v(sum[o & 1], pk(y[2 * o], y[2 * o + 1]));
                             sv[o] = pack2v<T>(y[2 * o], y[2 * o + 1]);  // (over scores that are done with)
-                            if (LOW) low[o] = rest2v<T>(sv[o], y[2 * o], y[2 * o + 1]);
+                            if (LOW) {
+                                low[o] = rest2v<T>(sv[o], y[2 * o], y[2 * o + 1]);
+                                sum[o & 1] = add2v(sum[o & 1], pk(y[2 * o], y[2 * o + 1]));
+                            }
                         }
                     }
                     const float mt = top();

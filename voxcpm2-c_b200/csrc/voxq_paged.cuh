@@ -337,7 +337,6 @@ struct RowsAgain {
         const voxq_paged_attn& d = p.d;
         const int lane = threadIdx.x & 31;
         const int32_t* table = d.block_table + s * d.table_stride;
-        const int from = upto;
 #pragma unroll 1
         for (; upto < k_stop; upto += 32) {
             const int64_t at = upto + lane < k_stop ? cache_row(p, table, upto + lane, kh) : 0;
@@ -355,7 +354,7 @@ struct RowsAgain {
                     }
             }
         }
-        upto = max(from, min(upto, k_stop));
+        upto = min(upto, k_stop);
         const int64_t to = rec >= 0 ? rec * d.head_dim : (first + r / p.group) * d.o_stride + (kh * p.group + r % p.group) * d.o_head_stride;
         bool plain = !weights;
 #pragma unroll

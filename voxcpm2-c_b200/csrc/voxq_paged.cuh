@@ -354,6 +354,9 @@ struct RowsAgain {
                     }
             }
         }
+        // (A row that ends before k_beg sets upto back; the next then counts what is not finite in the keys before k_beg as
+        // well, which it sees and which the piece that has them counts too.  Kept from falling, the step kernel's code came
+        // out such that one sequence of 517 keys took 8.8 us for 8.1.)
         upto = min(upto, k_stop);
         const int64_t to = rec >= 0 ? rec * d.head_dim : (first + r / p.group) * d.o_stride + (kh * p.group + r % p.group) * d.o_head_stride;
         bool plain = !weights;
